@@ -369,6 +369,65 @@ int prl_rope(const void* q, void* q_out, const int64_t* q_strides, int64_t q_hea
              int64_t cs_token_stride, int dtype, int64_t B, int64_t T, int64_t D, int inverse, void* stream);
 
 /*
+ * Rotary position embedding of query and key from position ids, in one launch.  Pair j < r / 2 of a head
+ * (r = rotary_dim) turns by the angle positions[b, t] * inv_freq[j] with amplitude a:
+ *     u' = a (u cos - v sin),  v' = a (v cos + u sin);   inverse = 1: the transpose (the backward on the gradients)
+ * (u, v) = (x[j], x[j + r/2]), or with interleaved = 1 (x[2j], x[2j + 1]); x[i], i >= r, is copied.  Angles are formed
+ * in fp64 (a far position's angle does not fit fp32), the rotation in fp32, each output is rounded once.
+ * Stretching for long contexts is in the inverse frequencies and the amplitude the caller brings.  Beside prl_rope,
+ * which takes cos / sin tables (src/prime_rl/trainer/model.py:74-75 is the reference's switch for such kernels).
+ *   q [B, q_heads, T, D], k [B, k_heads, T, D] (k_heads = 0: none, k may be NULL), any strides, last dimension
+ *   contiguous, element-aligned; q_strides / k_strides are HOST arrays of 6 element strides (batch, head, token of
+ *   the input, then of the output).  q_out / k_out may be q / k themselves under equal strides.
+ *   positions  int64 (positions_64 = 1) or int32, element strides over batch and token (a batch stride of 0 is fine)
+ *   inv_freq   fp32 or (inv_freq_64 = 1) fp64 [r / 2], contiguous
+ * Limits: r even, 2 <= r <= min(D, 8192) (prl_rope_positions_supported), B * T < 2^31 - 64.
+ */
+int prl_rope_positions_supported(int dtype, int64_t D, int64_t rotary_dim);
+int prl_rope_positions(const void* q, void* q_out, const int64_t* q_strides, int64_t q_heads, const void* k, void* k_out,
+                       const int64_t* k_strides, int64_t k_heads, const void* positions, int positions_64,
+                       int64_t pos_batch_stride, int64_t pos_token_stride, const void* inv_freq, int inv_freq_64,
+                       int64_t rotary_dim, int interleaved, float amplitude, int dtype, int64_t B, int64_t T, int64_t D,
+                       int inverse, void* stream);
+
+/*
+ * The norm behind a block's branch, its gate and residual scale, the addition, and the norm before the next block:
+ *     n = branch * rsqrt(mean(branch^2) + eps_post) * (w_post + weight_offset)     (w_post NULL: n = branch)
+ *     hidden = x + scale * gate * n
+ *     normed = hidden * rsqrt(mean(hidden^2) + eps_pre) * (w_pre + weight_offset)   (w_pre NULL: not formed)
+ * for layers with a norm on either side of a block, gated or scaled residuals; beside prl_add_rmsnorm_*, which has
+ * the addition and the norm after it (the switch `model.impl = "liger_kernel"`, src/prime_rl/trainer/model.py:74-75).
+ * All in fp32, each output rounded once: normed is formed from the unrounded hidden, unlike prl_add_rmsnorm_fwd.
+ * Every tensor shares `dtype`; rows of H elements with element strides between rows, any alignment of an element
+ * (multiples of 16 bytes are faster); 1 <= H <= 8192 (prl_block_norms_supported).
+ *   gate_kind  PRL_GATE_NONE | _CHANNEL (gate [H]) | _TOKEN (one per row, gate_stride apart) | _FULL (rows of H) |
+ *              _ONE (one value)
+ *   rstd_post, rstd_pre  fp32 [rows], written for the backward where their weight is given; NULL to skip
+ * Backward: g_hidden (NULL = 0) and g_normed (with w_pre) come in; gx and g_branch are written, and where not NULL
+ * g_w_post, g_w_pre [H] and g_gate in the gate's shape (g_gate_stride between rows), summed over rows in a fixed
+ * order.  workspace: prl_block_norms_bwd_workspace_bytes, 16-byte aligned; needed for any of the sums over rows.
+ */
+#define PRL_GATE_NONE 0
+#define PRL_GATE_CHANNEL 1
+#define PRL_GATE_TOKEN 2
+#define PRL_GATE_FULL 3
+#define PRL_GATE_ONE 4
+int prl_block_norms_supported(int dtype, int64_t H);
+size_t prl_block_norms_bwd_workspace_bytes(int dtype, int64_t rows, int64_t H);
+int prl_block_norms_fwd(const void* x, int64_t x_stride, const void* branch, int64_t branch_stride, const void* w_post,
+                        const void* w_pre, int gate_kind, const void* gate, int64_t gate_stride, float scale,
+                        float weight_offset, float eps_post, float eps_pre, void* hidden, int64_t hidden_stride,
+                        void* normed, int64_t normed_stride, float* rstd_post, float* rstd_pre, int dtype, int64_t rows,
+                        int64_t H, void* stream);
+int prl_block_norms_bwd(const void* x, int64_t x_stride, const void* branch, int64_t branch_stride, const void* w_post,
+                        const void* w_pre, int gate_kind, const void* gate, int64_t gate_stride, float scale,
+                        float weight_offset, const float* rstd_post, const float* rstd_pre, const void* g_hidden,
+                        int64_t g_hidden_stride, const void* g_normed, int64_t g_normed_stride, void* gx,
+                        int64_t gx_stride, void* g_branch, int64_t g_branch_stride, void* g_w_post, void* g_w_pre,
+                        void* g_gate, int64_t g_gate_stride, int dtype, int64_t rows, int64_t H, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/*
  * out = silu(gate) * up over n contiguous elements, and the backward
  *   gup = gout * silu(gate),  ggate = gout * up * silu'(gate).
  * The gated MLP activation of the transformer blocks; third kernel of the
@@ -481,6 +540,36 @@ int prl_attn_long_bwd(const void* q, const int64_t* q_strides, const void* k, co
 int prl_adamw_flat(float* param, float* grad, float* exp_avg, float* exp_avg_sq, void* compute_copy, int copy_dtype,
                    int64_t n, const float* grad_scale, int zero_grad, float lr, float beta1, float beta2, float eps,
                    float weight_decay, int64_t step, void* stream);
+
+/*
+ * Global norm of many gradient tensors, and their scaling by min(1, max_norm / (norm + 1e-6)): the two halves of
+ * torch.nn.utils.clip_grad_norm_ as the reference calls it (src/prime_rl/trainer/rl/train.py:336-338).
+ * `pieces` is a HOST array (copied into the launches): contiguous runs of elements, fp32 or bf16 mixed, any alignment
+ * of an element; no two may overlap in a prl_grad_scale call.
+ *   kind      PRL_NORM_L2 or PRL_NORM_MAX
+ *   total     double [1]: sum of squares or largest magnitude (what ranks add up or take the maximum of); may be NULL
+ *   norm      fp32 [1], may be NULL;  coef  fp32 [1], the factor, may be NULL
+ *   workspace prl_grad_norm_workspace_bytes(pieces, n_pieces), 8-byte aligned
+ * prl_grad_norm_finish joins n_parts partial totals (e.g. the one all ranks have reduced) and gives total, norm and
+ * coef.  prl_grad_scale multiplies every piece by coef[0] in place; where that is exactly 1 nothing is touched.
+ * Squares are added in fp64 in an order fixed by the sizes.  A NaN anywhere gives NaN, an infinity an infinite norm.
+ */
+#define PRL_NORM_L2 0
+#define PRL_NORM_MAX 1
+
+typedef struct prl_grad_piece {
+  void* x;       /* device */
+  int64_t n;     /* elements */
+  int32_t dtype; /* PRL_F32 or PRL_BF16 */
+  int32_t reserved;
+} prl_grad_piece;
+
+size_t prl_grad_norm_workspace_bytes(const prl_grad_piece* pieces, int64_t n_pieces);
+int prl_grad_norm(const prl_grad_piece* pieces, int64_t n_pieces, int kind, float max_norm, double* total, float* norm,
+                  float* coef, void* workspace, size_t workspace_bytes, void* stream);
+int prl_grad_norm_finish(const double* parts, int64_t n_parts, int kind, float max_norm, double* total, float* norm,
+                         float* coef, void* stream);
+int prl_grad_scale(const prl_grad_piece* pieces, int64_t n_pieces, const float* coef, void* stream);
 
 /*
  * Query / key RMSNorm over every head followed by the rotary embedding, reading the query and key blocks of a

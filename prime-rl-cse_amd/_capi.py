@@ -19,12 +19,20 @@ RATIO_TOKEN, RATIO_SEQUENCE = 0, 1
 ADVANTAGE_KIND = {"drgrpo": 0, "drgrpo-negclipped": 1, "rloo": 2, "opo": 3}
 
 STAT_IDENTITY, STAT_EXP = 0, 1
+GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL, GATE_ONE = 0, 1, 2, 3, 4
+NORM_L2, NORM_MAX = 0, 1
 
 
 class StatPiece(Structure):
     """prl_stat_piece of include/prl_hip.h."""
 
     _fields_ = [("x", c_void_p), ("mask", c_void_p), ("n", c_int64), ("key", c_int32), ("op", c_int32)]
+
+
+class GradPiece(Structure):
+    """prl_grad_piece of include/prl_hip.h."""
+
+    _fields_ = [("x", c_void_p), ("n", c_int64), ("dtype", c_int32), ("reserved", c_int32)]
 
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libprl_hip.so"
@@ -161,6 +169,34 @@ SIGNATURES = {
         [c_void_p, c_void_p, POINTER(c_int64), c_int64, c_void_p, c_void_p, POINTER(c_int64), c_int64, c_void_p,
          c_void_p, c_int64, c_int64, c_int, c_int64, c_int64, c_int64, c_int, c_void_p],
     ),
+    "prl_rope_positions_supported": (c_int, [c_int, c_int64, c_int64]),
+    "prl_rope_positions": (
+        c_int,
+        [c_void_p, c_void_p, POINTER(c_int64), c_int64, c_void_p, c_void_p, POINTER(c_int64), c_int64, c_void_p, c_int,
+         c_int64, c_int64, c_void_p, c_int, c_int64, c_int, c_float, c_int, c_int64, c_int64, c_int64, c_int, c_void_p],
+    ),
+    "prl_block_norms_supported": (c_int, [c_int, c_int64]),
+    "prl_block_norms_bwd_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64]),
+    "prl_block_norms_fwd": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_float, c_float, c_float,
+         c_float, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p],
+    ),
+    "prl_block_norms_bwd": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_float, c_float, c_void_p,
+         c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+         c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_size_t, c_void_p],
+    ),
+    "prl_grad_norm_workspace_bytes": (c_size_t, [POINTER(GradPiece), c_int64]),
+    "prl_grad_norm": (
+        c_int,
+        [POINTER(GradPiece), c_int64, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    "prl_grad_norm_finish": (
+        c_int, [c_void_p, c_int64, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "prl_grad_scale": (c_int, [POINTER(GradPiece), c_int64, c_void_p, c_void_p]),
     "prl_rmsnorm_supported": (c_int, [c_int, c_int64]),
     "prl_rmsnorm_bwd_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64]),
     "prl_rmsnorm_fwd": (

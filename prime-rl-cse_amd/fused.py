@@ -20,6 +20,7 @@ from typing import Any
 
 import torch
 from torch import Tensor, nn
+from torch.autograd.function import once_differentiable
 
 from . import _capi as C
 from . import lm_head
@@ -196,6 +197,130 @@ def add_rms_norm(x: Tensor, branch: Tensor, weight: Tensor, eps: float) -> tuple
     return _AddRMSNorm.apply(x, branch, weight, float(eps))
 
 
+# --------------------------------------------------------------------------- norms before and after a block
+
+
+def _pitched(x: Tensor, h: int) -> Tensor:
+    """x as [rows, h] with the last dimension contiguous: a view where its layout allows one, else a copy."""
+    if x.ndim != 2:
+        x = x.reshape(-1, h)  # a view whenever the leading dimensions merge
+    if x.stride(1) != 1 and h > 1:
+        x = x.contiguous()
+    return x
+
+
+def _gate_rows(gate: Tensor, lead: tuple[int, ...], h: int) -> tuple[int, Tensor]:
+    """(kind, the gate as the kernels read it): [h], one value per row, [rows, h], or one value."""
+    if gate.shape == (*lead, h):
+        return C.GATE_FULL, _pitched(gate, h)
+    if gate.shape == (h,):
+        return C.GATE_CHANNEL, gate.contiguous()
+    if gate.shape == (*lead, 1):
+        return C.GATE_TOKEN, gate.reshape(-1)
+    if gate.ndim <= 1 and gate.numel() == 1:
+        return C.GATE_ONE, gate.reshape(1)
+    raise ValueError(f"block_norms: a gate of shape {tuple(gate.shape)} for rows {lead} of {h}: one value, ({h},), "
+                     f"{(*lead, 1)} or {(*lead, h)} (expand others yourself)")
+
+
+class _BlockNorms(torch.autograd.Function):
+    """x, branch [rows, h] and the gate in one of its three layouts; see `block_norms`."""
+
+    @staticmethod
+    def forward(ctx, x: Tensor, branch: Tensor, w_post: Tensor | None, w_pre: Tensor | None, gate: Tensor | None,
+                kind: int, scale: float, offset: float, eps_post: float, eps_pre: float):
+        dev = x.device
+        rows, h = x.shape
+        train = any(ctx.needs_input_grad)
+        hidden = torch.empty((rows, h), dtype=x.dtype, device=dev)
+        normed = None if w_pre is None else torch.empty((rows, h), dtype=x.dtype, device=dev)
+        r1 = torch.empty(rows, dtype=torch.float32, device=dev) if train and w_post is not None else None
+        r2 = torch.empty(rows, dtype=torch.float32, device=dev) if train and w_pre is not None else None
+        with C.on_device(dev), C.timed("prl_block_norms_fwd", dev):
+            C.check(C.load().prl_block_norms_fwd(
+                C.ptr(x), x.stride(0), C.ptr(branch), branch.stride(0), C.ptr(w_post), C.ptr(w_pre), kind, C.ptr(gate),
+                0 if gate is None else gate.stride(0), scale, offset, eps_post, eps_pre, C.ptr(hidden), h,
+                C.ptr(normed), h, C.ptr(r1), C.ptr(r2), C.dtype_code(x), rows, h, C.stream_ptr(dev)),
+                "prl_block_norms_fwd")
+        ctx.save_for_backward(x, branch, w_post, w_pre, gate, r1, r2)
+        ctx.args = (kind, scale, offset)
+        ctx.set_materialize_grads(False)
+        return hidden, normed
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gh: Tensor | None, gy: Tensor | None):
+        x, branch, w_post, w_pre, gate, r1, r2 = ctx.saved_tensors
+        kind, scale, offset = ctx.args
+        if gh is None and gy is None:
+            return (None,) * 10
+        dev = x.device
+        lib = C.load()
+        rows, h = x.shape
+        if gy is None:  # the normalised output went nowhere
+            w_pre = r2 = None
+        gh = None if gh is None else _pitched(gh, h)
+        gy = None if gy is None else _pitched(gy, h)
+        need = ctx.needs_input_grad
+        gx, gb = torch.empty((rows, h), dtype=x.dtype, device=dev), torch.empty((rows, h), dtype=x.dtype, device=dev)
+        g1 = torch.empty_like(w_post) if w_post is not None and need[2] else None
+        g2 = torch.empty_like(w_pre) if w_pre is not None and need[3] else None
+        gg = torch.empty(gate.shape, dtype=x.dtype, device=dev) if gate is not None and need[4] else None
+        code = C.dtype_code(x)
+        ws = None
+        if g1 is not None or g2 is not None or (gg is not None and kind in (C.GATE_CHANNEL, C.GATE_ONE)):
+            ws = torch.empty(lib.prl_block_norms_bwd_workspace_bytes(code, rows, h), dtype=torch.uint8, device=dev)
+        with C.on_device(dev), C.timed("prl_block_norms_bwd", dev):
+            C.check(lib.prl_block_norms_bwd(
+                C.ptr(x), x.stride(0), C.ptr(branch), branch.stride(0), C.ptr(w_post), C.ptr(w_pre), kind, C.ptr(gate),
+                0 if gate is None else gate.stride(0), scale, offset, C.ptr(r1), C.ptr(r2), C.ptr(gh),
+                0 if gh is None else gh.stride(0), C.ptr(gy), 0 if gy is None else gy.stride(0), C.ptr(gx), h, C.ptr(gb),
+                h, C.ptr(g1), C.ptr(g2), C.ptr(gg), 0 if gg is None else gg.stride(0), code, rows, h, C.ptr(ws),
+                0 if ws is None else ws.numel(), C.stream_ptr(dev)), "prl_block_norms_bwd")
+        return gx, gb, g1, g2, gg, None, None, None, None, None
+
+
+def block_norms_supported(x: Tensor, branch: Tensor, post_weight: Tensor | None = None, pre_weight: Tensor | None = None,
+                          gate: Tensor | None = None) -> bool:
+    """Whether `block_norms` takes these tensors: one dtype (bf16 or fp32), one HIP device, rows of at most 8192."""
+    given = [t for t in (branch, post_weight, pre_weight, gate) if t is not None]
+    if not x.is_cuda or x.ndim < 1 or x.dtype not in (torch.bfloat16, torch.float32) or x.shape != branch.shape \
+            or any(t.dtype != x.dtype or t.device != x.device or hasattr(t, "to_local") for t in given):
+        return False
+    h = x.shape[-1]
+    return 1 <= h <= 8192 and all(w is None or w.shape == (h,) for w in (post_weight, pre_weight))
+
+
+def block_norms(x: Tensor, branch: Tensor, post_weight: Tensor | None = None, pre_weight: Tensor | None = None, *,
+                gate: Tensor | None = None, scale: float = 1.0, eps: float = 1e-6, pre_eps: float | None = None,
+                weight_offset: float = 0.0) -> tuple[Tensor, Tensor | None]:
+    """(hidden, normed) with
+
+        hidden = x + scale * gate * rms(branch, eps) * (post_weight + weight_offset)
+        normed = rms(hidden, pre_eps) * (pre_weight + weight_offset),      rms(v, e) = v * rsqrt(mean(v^2, -1) + e)
+
+    in one launch, differentiable in all five tensors: what a layer does between a block's output and the next
+    block's input when it normalises, gates or scales the branch.  Without `post_weight` the branch is added as it is;
+    without `pre_weight` normed is None.  `gate` is one value, one per channel [H], per row [..., 1] or per element
+    (x's shape).  `pre_eps` defaults to `eps`.  fp32 inside, each output rounded once; `normed` is
+    formed from the unrounded hidden (`add_rms_norm` rounds the sum first, as separate modules do)."""
+    dev = C.require_device(x, branch, post_weight, pre_weight, gate)
+    if not block_norms_supported(x, branch, post_weight, pre_weight, gate):
+        raise ValueError("block_norms: x and branch of one shape with rows of 1 to 8192, weights of a row's length, all "
+                         f"in one dtype (bf16 or fp32); got x {tuple(x.shape)} {x.dtype}, branch {tuple(branch.shape)} "
+                         f"{branch.dtype}, weights " + ", ".join("none" if w is None else f"{tuple(w.shape)} {w.dtype}"
+                                                                 for w in (post_weight, pre_weight)) + " on " + str(dev))
+    h, lead = x.shape[-1], tuple(x.shape[:-1])
+    kind = C.GATE_NONE
+    if gate is not None:
+        kind, gate = _gate_rows(gate, lead, h)
+    w1 = None if post_weight is None else post_weight.contiguous()
+    w2 = None if pre_weight is None else pre_weight.contiguous()
+    hidden, normed = _BlockNorms.apply(_pitched(x, h), _pitched(branch, h), w1, w2, gate, kind, float(scale),
+                                       float(weight_offset), float(eps), float(eps if pre_eps is None else pre_eps))
+    return hidden.view(x.shape), None if normed is None else normed.view(x.shape)
+
+
 # --------------------------------------------------------------------------- rotary position embedding
 
 
@@ -263,6 +388,182 @@ def apply_rotary_pos_emb(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, unsquee
     if unsqueeze_dim == 1 and rope_supported(q, k, cos, sin):
         return _Rope.apply(q, k, cos, sin)
     return _ORIGINAL_ROPE[0](q, k, cos, sin, unsqueeze_dim)
+
+
+
+def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict[str, Any] | None = None,
+                     max_position_embeddings: int | None = None, seq_len: int | None = None,
+                     device: torch.device | str | None = None) -> tuple[Tensor, float]:
+    """(inverse frequencies fp32 [rotary_dim / 2], amplitude of cos and sin) for `rope_at_positions`: base^(-2 j / r),
+    stretched for long contexts as `scaling` says, a dict with a checkpoint config's keys (`rope_type` and its
+    parameters).  Formed in fp64 and rounded once.
+
+      "default"
+      "linear"    all frequencies divided by `factor` (positions interpolated)
+      "dynamic"   the base grows with the length once `seq_len` exceeds max_position_embeddings (NTK-aware)
+      "yarn"      a ramp over the pairs between full turns `beta_fast` and `beta_slow` within the original context:
+                  fast pairs kept, slow ones divided by `factor`; amplitude 0.1 ln(factor) + 1
+      "llama3"    the same with the ramp over wavelengths (`low_freq_factor`, `high_freq_factor`)
+      "longrope"  a factor per pair, `short_factor` or (seq_len beyond the original context) `long_factor`"""
+    import math
+
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rope_frequencies: rotary_dim must be even and at least 2, got {rotary_dim}")
+    sc = dict(scaling or {})
+    kind = sc.get("rope_type", sc.get("type", "default"))
+    base = float(sc.get("rope_theta", base))
+    r = rotary_dim
+    j = torch.arange(r // 2, dtype=torch.float64)
+
+    def need(key: str) -> Any:
+        if sc.get(key) is None:
+            raise ValueError(f"rope_frequencies: rope_type {kind!r} needs {key!r}")
+        return sc[key]
+
+    def context() -> float:
+        n = sc.get("original_max_position_embeddings") or max_position_embeddings
+        if not n:
+            raise ValueError(f"rope_frequencies: rope_type {kind!r} needs max_position_embeddings")
+        return float(n)
+
+    amplitude = 1.0
+    if kind == "dynamic":
+        n, factor = context(), float(need("factor"))
+        length = max(float(seq_len or 0), n)
+        if r > 2:
+            base = base * (factor * length / n - (factor - 1.0)) ** (r / (r - 2.0))
+    freq = base ** (-2.0 * j / r)
+    if kind == "linear":
+        freq = freq / float(need("factor"))
+    elif kind == "yarn":
+        n = context()
+        factor = float(sc.get("factor") or (max_position_embeddings or n) / n)
+
+        def pair_with(turns: float) -> float:  # the (fractional) pair that turns this often within the context
+            return r * math.log(n / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
+
+        low, high = pair_with(float(sc.get("beta_fast") or 32.0)), pair_with(float(sc.get("beta_slow") or 1.0))
+        if sc.get("truncate", True):
+            low, high = math.floor(low), math.ceil(high)
+        low, high = max(low, 0), min(high, r - 1)
+        ramp = ((j - low) / (high - low if high != low else 0.001)).clamp(0.0, 1.0)
+        freq = freq * (1.0 - ramp) + freq / factor * ramp
+
+        def magnitude(m: float) -> float:
+            return 1.0 if factor <= 1.0 else 0.1 * m * math.log(factor) + 1.0
+
+        if sc.get("attention_factor") is not None:
+            amplitude = float(sc["attention_factor"])
+        elif sc.get("mscale") and sc.get("mscale_all_dim"):
+            amplitude = magnitude(float(sc["mscale"])) / magnitude(float(sc["mscale_all_dim"]))
+        else:
+            amplitude = magnitude(1.0)
+    elif kind == "llama3":
+        n, factor = context(), float(need("factor"))
+        lo, hi = float(need("low_freq_factor")), float(need("high_freq_factor"))
+        keep = ((n * freq / (2.0 * math.pi) - lo) / (hi - lo)).clamp(0.0, 1.0)
+        freq = freq * keep + freq / factor * (1.0 - keep)
+    elif kind == "longrope":
+        n = context()
+        which = "long_factor" if seq_len and seq_len > n else "short_factor"
+        per_pair = torch.tensor(need(which), dtype=torch.float64)
+        if per_pair.numel() != r // 2:
+            raise ValueError(f"rope_frequencies: {which} has {per_pair.numel()} entries for {r // 2} pairs")
+        freq = freq / per_pair
+        factor = float(sc.get("factor") or (max_position_embeddings or n) / n)
+        if sc.get("attention_factor") is not None:
+            amplitude = float(sc["attention_factor"])
+        elif factor > 1.0:
+            amplitude = math.sqrt(1.0 + math.log(factor) / math.log(n))
+    elif kind not in ("default", "dynamic"):
+        raise ValueError(f"rope_frequencies: unknown rope_type {kind!r}")
+    return freq.to(torch.float32).to(device) if device is not None else freq.to(torch.float32), amplitude
+
+
+def _launch_rope_positions(q: Tensor | None, k: Tensor | None, pos: Tensor, inv_freq: Tensor, interleaved: bool,
+                           amplitude: float, inverse: bool) -> tuple[Tensor | None, Tensor | None]:
+    """Either of q and k may be None.  Outputs keep their inputs' strides where those are dense."""
+    one = q if q is not None else k
+    dev = one.device
+    b, _, t, d = one.shape
+    args = []
+    outs = []
+    q, k = (x if x is None or x.stride(3) == 1 else x.contiguous() for x in (q, k))  # (both alive until the launch)
+    for x in (q, k):
+        if x is None:
+            outs.append(None)
+            args += [None, None, None, 0]
+            continue
+        out = torch.empty_like(x)
+        outs.append(out)
+        args += [x.data_ptr(), out.data_ptr(), _strides6(x, out), x.shape[1]]
+    if 0 in (b, t) or args[3] + args[7] == 0:
+        return outs[0], outs[1]
+    with C.on_device(dev), C.timed("prl_rope_positions", dev):
+        C.check(C.load().prl_rope_positions(
+            *args, pos.data_ptr(), pos.dtype == torch.int64, pos.stride(0) if pos.shape[0] > 1 else 0, pos.stride(1),
+            inv_freq.data_ptr(), inv_freq.dtype == torch.float64, 2 * inv_freq.numel(), interleaved, amplitude,
+            C.dtype_code(one), b, t, d, inverse, C.stream_ptr(dev)), "prl_rope_positions")
+    return outs[0], outs[1]
+
+
+class _RopePositions(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q: Tensor, k: Tensor | None, pos: Tensor, inv_freq: Tensor, interleaved: bool, amplitude: float):
+        ctx.save_for_backward(pos, inv_freq)
+        ctx.args = (interleaved, amplitude)
+        ctx.set_materialize_grads(False)
+        return _launch_rope_positions(q, k, pos, inv_freq, interleaved, amplitude, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq: Tensor | None, gk: Tensor | None):
+        gq = gq if ctx.needs_input_grad[0] else None
+        gk = gk if ctx.needs_input_grad[1] else None
+        if gq is not None or gk is not None:
+            pos, inv_freq = ctx.saved_tensors
+            gq, gk = _launch_rope_positions(gq, gk, pos, inv_freq, *ctx.args, True)
+        return gq, gk, None, None, None, None
+
+
+def rope_at_positions_supported(q: Tensor, k: Tensor | None, position_ids: Tensor, inv_freq: Tensor) -> bool:
+    """Whether `rope_at_positions` takes these tensors."""
+    if q.ndim != 4 or not q.is_cuda or q.dtype not in (torch.bfloat16, torch.float32):
+        return False
+    b, _, t, d = q.shape
+    if k is not None and (k.ndim != 4 or k.dtype != q.dtype or k.device != q.device
+                          or (k.shape[0], k.shape[2], k.shape[3]) != (b, t, d)):
+        return False
+    if position_ids.dtype not in (torch.int64, torch.int32) or position_ids.device != q.device \
+            or tuple(position_ids.shape) not in ((b, t), (1, t), (t,)):
+        return False
+    return inv_freq.ndim == 1 and inv_freq.dtype in (torch.float32, torch.float64) and inv_freq.device == q.device \
+        and not inv_freq.requires_grad and 1 <= inv_freq.numel() and 2 * inv_freq.numel() <= min(d, 8192) \
+        and b * t < 2**31 - 64
+
+
+def rope_at_positions(q: Tensor, k: Tensor | None, position_ids: Tensor, inv_freq: Tensor, *, interleaved: bool = False,
+                      attention_scaling: float = 1.0) -> tuple[Tensor, Tensor | None]:
+    """Rotary embedding of q [B, heads, T, D] and k (or None) from position ids, one launch, differentiable in both.
+
+    The first 2 * len(inv_freq) dimensions of every head turn by position * inv_freq[j], the others pass through; pair
+    j is (x[j], x[j + len(inv_freq)]), or with `interleaved` (x[2j], x[2j + 1]).  `attention_scaling` multiplies cos
+    and sin.  `position_ids` [B, T], [1, T] or [T] (int64 or int32) need not be in order; angles are formed in fp64,
+    so far positions keep their fraction of a turn.  `inv_freq` (fp32 or fp64) as `rope_frequencies` or a model's
+    rotary module gives it.  No cos / sin tables are read or kept for the backward.  Any strides; q and k as blocks of
+    a stacked projection are taken where they lie."""
+    C.require_device(q, k, position_ids, inv_freq)
+    if not rope_at_positions_supported(q, k, position_ids, inv_freq):
+        raise ValueError(
+            "rope_at_positions: q [B, heads, T, D] and k [B, heads, T, D] or None in one dtype (bf16 or fp32), position_ids "
+            "[B, T], [1, T] or [T] int64 or int32, inv_freq [r / 2] fp32 or fp64 without gradient, r <= min(D, 8192); got q "
+            f"{tuple(q.shape)} {q.dtype}, k {None if k is None else (tuple(k.shape), k.dtype)}, position_ids "
+            f"{tuple(position_ids.shape)} {position_ids.dtype}, inv_freq {tuple(inv_freq.shape)} {inv_freq.dtype}")
+    pos = position_ids if position_ids.ndim == 2 else position_ids.unsqueeze(0)
+    inv_freq = inv_freq.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _RopePositions.apply(q, k, pos, inv_freq, bool(interleaved), float(attention_scaling))
+    return _launch_rope_positions(q, k, pos, inv_freq, bool(interleaved), float(attention_scaling), False)
 
 
 # --------------------------------------------------------------------------- SwiGLU

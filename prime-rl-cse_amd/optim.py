@@ -90,6 +90,167 @@ def setup_optimizer(config: Any, model: nn.Module, fused: bool | None = None, fl
     raise ValueError(f"Invalid optimizer type: {config.type}")
 
 
+# --------------------------------------------------------------------------- gradient norm and clipping
+
+
+def _local(g: torch.Tensor) -> torch.Tensor:
+    return g.to_local() if hasattr(g, "to_local") else g
+
+
+def _sharding(grads: list[torch.Tensor]) -> list[Any] | None:
+    """Process groups over which the squares of these gradients' local parts have to be added up: those of the mesh
+    dimensions the gradients are sharded over ([] for plain tensors and for meshes of one rank).  None if they are
+    not all plain, or all DTensors of one mesh with one placement, sharded or replicated, per mesh dimension."""
+    spread = [g for g in grads if hasattr(g, "to_local")]
+    if not spread:
+        return []
+    mesh, kinds = spread[0].device_mesh, [p.is_shard() for p in spread[0].placements]
+    for g in grads:
+        if not hasattr(g, "to_local") or g.device_mesh != mesh or [p.is_shard() for p in g.placements] != kinds \
+                or any(p.is_partial() for p in g.placements):
+            return None
+    return [mesh.get_group(i) for i, shard in enumerate(kinds) if shard and mesh.size(i) > 1]
+
+
+def _is_one_run(g: torch.Tensor) -> bool:
+    """Whether a tensor's elements fill one run of memory, in whatever order of its dimensions."""
+    if g.is_contiguous():
+        return True
+    at = 1
+    for stride, size in sorted((st, n) for st, n in zip(g.stride(), g.shape) if n != 1):
+        if stride != at:
+            return False
+        at *= size
+    return True
+
+
+def clip_grad_norm_supported(grads: list[torch.Tensor]) -> bool:
+    """Whether `clip_grad_norm_` takes these gradients: bf16 or fp32, each one run of memory, on one HIP device, plain or
+    DTensors of one mesh that are sharded or replicated alike."""
+    if not grads:
+        return True
+    if _sharding(grads) is None:
+        return False
+    parts = [_local(g) for g in grads]
+    dev = parts[0].device
+    return dev.type == "cuda" and all(g.layout == torch.strided and g.device == dev and _is_one_run(g)
+                                      and g.dtype in (torch.float32, torch.bfloat16) for g in parts)
+
+
+def _pieces(grads: list[torch.Tensor], in_place: bool) -> tuple[Any, int]:
+    """The gradients as runs of memory: a `GradPiece` array and its length.  Runs that touch end to end become one."""
+    from . import _capi as C
+
+    runs: list[list[int]] = []
+    end, last = -1, None
+    for g in grads:
+        n = g.numel()
+        if n == 0:
+            continue
+        if g.layout != torch.strided or g.dtype not in (torch.float32, torch.bfloat16) or not _is_one_run(g):
+            raise ValueError("gradients must be dense float32 or bfloat16 tensors that fill one run of memory, got "
+                             f"{g.dtype} {g.layout} of shape {tuple(g.shape)}" +
+                             (f" with strides {g.stride()}" if g.layout == torch.strided else ""))
+        at, dtype = g.data_ptr(), g.dtype
+        if at == end and dtype is last:
+            runs[-1][1] += n
+        else:
+            runs.append([at, n, C.dtype_code(g)])
+            last = dtype
+        end = at + n * (4 if dtype is torch.float32 else 2)
+    if in_place and len(runs) > 1:
+        order = sorted(runs)
+        for a, b in zip(order, order[1:]):
+            if a[0] + a[1] * (4 if a[2] == C.PRL_F32 else 2) > b[0]:
+                raise ValueError("clip_grad_norm_: two gradients share memory (a parameter given twice?)")
+    return (C.GradPiece * max(len(runs), 1))(*[(x, n, d, 0) for x, n, d in runs]), len(runs)
+
+
+def _norm_kind(norm_type: float) -> int:
+    from . import _capi as C
+
+    if float(norm_type) == 2.0:
+        return C.NORM_L2
+    if float(norm_type) == math.inf:
+        return C.NORM_MAX
+    raise ValueError(f"norm_type must be 2 or inf, got {norm_type}")
+
+
+def _norm_and_factor(table: Any, n: int, dev: torch.device, kind: int, max_norm: float,
+                     groups: list[Any]) -> torch.Tensor:
+    """fp32 [2] on the device: the norm over `groups` and the clipping factor."""
+    from . import _capi as C
+    from .utils import _all_reduce
+
+    lib = C.load()
+    out = torch.empty(2, dtype=torch.float32, device=dev)
+    size = lib.prl_grad_norm_workspace_bytes(table, n)
+    ws = torch.empty(size // 8 + 1, dtype=torch.float64, device=dev)  # the last one: the total
+    total = ws.data_ptr() + size
+    st = C.stream_ptr(dev)
+    C.check(lib.prl_grad_norm(table, n, kind, max_norm, total, out.data_ptr(), out.data_ptr() + 4, ws.data_ptr(), size,
+                              st), "prl_grad_norm")
+    if groups:
+        whole = ws[-1:]
+        for group in groups:
+            _all_reduce(whole, torch.distributed.ReduceOp.MAX if kind == C.NORM_MAX else torch.distributed.ReduceOp.SUM,
+                        group)
+        C.check(lib.prl_grad_norm_finish(total, 1, kind, max_norm, 0, out.data_ptr(), out.data_ptr() + 4, st),
+                "prl_grad_norm_finish")
+    return out
+
+
+@torch.no_grad()
+def grad_norm(grads: Any, norm_type: float = 2.0) -> torch.Tensor:
+    """The norm (2 or inf) of all these tensors together, an fp32 scalar on their device, as
+    torch.nn.utils.get_total_norm; squares are added in fp64 and nothing is copied to the host.  DTensors count with
+    all ranks' shards."""
+    from . import _capi as C
+
+    grads = list(grads)
+    kind = _norm_kind(norm_type)
+    if not grads:
+        return torch.tensor(0.0)
+    groups = _sharding(grads)
+    if groups is None:
+        raise ValueError("grad_norm: plain tensors, or DTensors of one mesh placed alike (sharded or replicated)")
+    parts = [_local(g) for g in grads]
+    dev = C.require_device(*parts)
+    table, n = _pieces(parts, in_place=False)
+    with C.on_device(dev), C.timed("prl_grad_norm", dev):
+        return _norm_and_factor(table, n, dev, kind, 0.0, groups)[0]
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: Any, max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """torch.nn.utils.clip_grad_norm_ (src/prime_rl/trainer/rl/train.py:336-338) on the package's kernels: every
+    gradient is multiplied in place by min(1, max_norm / (norm + 1e-6)); returns the norm before, an fp32 scalar on the
+    device.  One read of the gradients for the norm; the second pass leaves them untouched when there is nothing to
+    clip.  No host synchronisation (`error_if_nonfinite` looks at the norm and has one).  FSDP2's sharded gradients
+    are taken with one all-reduced scalar per sharded mesh dimension.  bf16 and fp32 gradients may be mixed;
+    `norm_type` is 2 or inf; a gradient given twice, or sharing memory with another, is refused."""
+    from . import _capi as C
+
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in params if p.grad is not None]
+    kind = _norm_kind(norm_type)
+    if not grads:
+        return torch.tensor(0.0)
+    groups = _sharding(grads)
+    if groups is None:
+        raise ValueError("clip_grad_norm_: plain gradients, or DTensors of one mesh placed alike (sharded or replicated)")
+    parts = [_local(g) for g in grads]
+    dev = C.require_device(*parts)
+    table, n = _pieces(parts, in_place=True)
+    with C.on_device(dev), C.timed("prl_clip_grad_norm", dev):
+        out = _norm_and_factor(table, n, dev, kind, float(max_norm), groups)
+        if error_if_nonfinite and not math.isfinite(float(out[0])):
+            raise RuntimeError(f"The total norm of order {norm_type} of the gradients is not finite, so they cannot be clipped")
+        C.check(C.load().prl_grad_scale(table, n, out.data_ptr() + 4, C.stream_ptr(dev)), "prl_grad_scale")
+    return out[0]
+
+
 def _floor_factor(lr: float, min_lr: float) -> float:
     return min_lr / lr if min_lr > 0 else 1e-8
 

@@ -80,15 +80,15 @@ def flexible_all_gather(tensor: Tensor) -> Tensor:
     return torch.cat([gathered[r * width : r * width + n] for r, n in enumerate(sizes)])
 
 
-def _all_reduce(t: Tensor, op) -> None:
+def _all_reduce(t: Tensor, op, group: Any = None) -> None:
     """In-place all-reduce of a device tensor.  RCCL ("nccl") reduces it where it
     is; any other backend (gloo in tests) gets a synchronous host copy, because
     gloo collectives on device tensors are not reliable when ranks share a GPU."""
-    if dist.get_backend() == "nccl":
-        dist.all_reduce(t, op=op)
+    if dist.get_backend(group) == "nccl":
+        dist.all_reduce(t, op=op, group=group)
         return
     host = t.cpu()
-    dist.all_reduce(host, op=op)
+    dist.all_reduce(host, op=op, group=group)
     t.copy_(host)
 
 
