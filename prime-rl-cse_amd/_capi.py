@@ -188,15 +188,15 @@ SIGNATURES = {
          c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
          c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_size_t, c_void_p],
     ),
-    "prl_grad_norm_workspace_bytes": (c_size_t, [POINTER(GradPiece), c_int64]),
+    "prl_grad_norm_workspace_bytes": (c_size_t, [c_void_p, c_int64]),
     "prl_grad_norm": (
         c_int,
-        [POINTER(GradPiece), c_int64, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
+        [c_void_p, c_int64, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
     ),
     "prl_grad_norm_finish": (
         c_int, [c_void_p, c_int64, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p],
     ),
-    "prl_grad_scale": (c_int, [POINTER(GradPiece), c_int64, c_void_p, c_void_p]),
+    "prl_grad_scale": (c_int, [c_void_p, c_int64, c_void_p, c_void_p]),
     "prl_rmsnorm_supported": (c_int, [c_int, c_int64]),
     "prl_rmsnorm_bwd_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64]),
     "prl_rmsnorm_fwd": (
@@ -308,8 +308,8 @@ class _OnDevice:
     __slots__ = ("ctx",)
 
     def __init__(self, device: torch.device):
-        self.ctx = None if device.index is None or torch.cuda.current_device() == device.index else \
-            torch.cuda.device(device)
+        index = device.index  # (a tensor's device exists, so the runtime is up: no need to ask for that first)
+        self.ctx = None if index is None or torch._C._cuda_getDevice() == index else torch.cuda.device(device)
 
     def __enter__(self):
         if self.ctx is not None:
@@ -326,7 +326,10 @@ def on_device(device: torch.device) -> _OnDevice:
 
 
 def stream_ptr(device: torch.device) -> c_void_p:
-    return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    """torch's current stream of the device.  By its raw handle: the Stream object that `torch.cuda.current_stream`
+    would make is 1.9 us of a call's host time, three times that in the autograd engine's thread."""
+    index = device.index
+    return c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice() if index is None else index))
 
 
 def ptr(t: torch.Tensor | None) -> c_void_p:

@@ -24,52 +24,86 @@
 namespace prl {
 
 constexpr int kBnMaxH = 8192;
-constexpr int kBnMaxBlocks = 1024;  // backward: also the number of partial rows the finish adds up
+constexpr int kBnRsrcFlags = 0x00020000;  // raw buffer, 32-bit data format (gfx9 family descriptor word 3)
 
-typedef unsigned int bn_v_e2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef unsigned int bn_v_e4 __attribute__((ext_vector_type(4), aligned(4)));
-
-// The VE elements of unit v of a row of H; with AL every unit is whole and 16-byte aligned, otherwise the address is
-// aligned to an element only and the last unit may be short (the rest reads as 0).
-template <int DT, bool AL>
-__device__ __forceinline__ void bn_load(const char* row, int v, int H, float* y) {
-  constexpr int ES = DT == PRL_F32 ? 4 : 2, VE = 16 / ES;
-  const char* p = row + (int64_t)v * 16;
-  const int left = H - v * VE;
-  if (AL || left >= VE) {
-    u32x4 z;
-    if constexpr (AL) z = *reinterpret_cast<const u32x4*>(p);
-    else if constexpr (DT == PRL_F32) z = *reinterpret_cast<const bn_v_e4*>(p);
-    else z = *reinterpret_cast<const bn_v_e2*>(p);
-    decode16_raw<DT>(z, y);
-    return;
+// A thread reads its share of a row in units of four registers.  VEC: a unit is 16 consecutive bytes, unit v at
+// 16 v, for rows whose every unit is whole and aligned.  Otherwise it is four single elements, `tpr` apart, so that a
+// wave's accesses lie side by side whatever the row's alignment: 16-byte accesses at odd places ran at half the
+// rate (8192 rows of 1531 bf16, a gate per element: forward 45.0 us against 31.8, backward 82.6 against 53.4).
+// Rows are read through descriptors of exactly their bytes: lanes beyond the end, and every lane of a tensor that is
+// not there, read 0 and store nothing, without a branch.
+template <int DT, bool VEC>
+struct BnUnit {
+  static constexpr int kEs = DT == PRL_F32 ? 4 : 2;
+  static constexpr int kN = VEC ? 16 / kEs : 4;  // elements
+  // column of element i of unit k of thread li
+  static __device__ __forceinline__ int column(int k, int i, int li, int tpr) {
+    return VEC ? (li + k * tpr) * kN + i : li + (k * kN + i) * tpr;
   }
+  static __device__ __forceinline__ u32x4 load(const char* row, int k, int li, int tpr, int H) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(row), 0, row ? H * kEs : 0, kBnRsrcFlags);
+    if constexpr (VEC) return __builtin_amdgcn_raw_buffer_load_b128(rsrc, (li + k * tpr) * 16, 0, 0);
+    uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < VE; ++i) {
-    y[i] = 0.0f;
-    if (i < left) y[i] = DT == PRL_F32 ? reinterpret_cast<const float*>(p)[i] : bf16_one(reinterpret_cast<const uint16_t*>(p)[i]);
-  }
-}
-template <int DT, bool AL>
-__device__ __forceinline__ void bn_store(char* row, int v, int H, const float* y) {
-  constexpr int ES = DT == PRL_F32 ? 4 : 2, VE = 16 / ES;
-  char* p = row + (int64_t)v * 16;
-  const int left = H - v * VE;
-  if (AL || left >= VE) {
-    u32x4 z;
-    if constexpr (DT == PRL_F32) {
-      z.x = __float_as_uint(y[0]), z.y = __float_as_uint(y[1]), z.z = __float_as_uint(y[2]), z.w = __float_as_uint(y[3]);
-    } else {
-      z.x = pack_bf16(y[0], y[1]), z.y = pack_bf16(y[2], y[3]), z.z = pack_bf16(y[4], y[5]), z.w = pack_bf16(y[6], y[7]);
+    for (int i = 0; i < 4; ++i) {
+      const int at = column(k, i, li, tpr) * kEs;
+      if constexpr (DT == PRL_F32) w[i] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, at, 0, 0);
+      else w[i] = __builtin_amdgcn_raw_buffer_load_b16(rsrc, at, 0, 0);
     }
-    if constexpr (AL) *reinterpret_cast<u32x4*>(p) = z;
-    else if constexpr (DT == PRL_F32) *reinterpret_cast<bn_v_e4*>(p) = z;
-    else *reinterpret_cast<bn_v_e2*>(p) = z;
-    return;
+    u32x4 z;
+    z.x = w[0], z.y = w[1], z.z = w[2], z.w = w[3];
+    return z;
   }
+  static __device__ __forceinline__ void decode(const u32x4& z, float* y) {
+    if constexpr (VEC || DT == PRL_F32) {
+      decode16_raw<DT>(z, y);
+    } else {
+      y[0] = bf16_lo(z.x), y[1] = bf16_lo(z.y), y[2] = bf16_lo(z.z), y[3] = bf16_lo(z.w);
+    }
+  }
+  static __device__ __forceinline__ void store(char* row, int k, int li, int tpr, int H, const float* y) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(row, 0, H * kEs, kBnRsrcFlags);
+    if constexpr (VEC) {
+      u32x4 z;
+      if constexpr (DT == PRL_F32) {
+        z.x = __float_as_uint(y[0]), z.y = __float_as_uint(y[1]), z.z = __float_as_uint(y[2]), z.w = __float_as_uint(y[3]);
+      } else {
+        z.x = pack_bf16(y[0], y[1]), z.y = pack_bf16(y[2], y[3]), z.z = pack_bf16(y[4], y[5]), z.w = pack_bf16(y[6], y[7]);
+      }
+      __builtin_amdgcn_raw_buffer_store_b128(z, rsrc, (li + k * tpr) * 16, 0, 0);
+    } else {
 #pragma unroll
-  for (int i = 0; i < VE; ++i)
-    if (i < left) store_elem<DT>(p, i, y[i]);
+      for (int i = 0; i < 4; ++i) {
+        const int at = column(k, i, li, tpr) * kEs;
+        if constexpr (DT == PRL_F32) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(y[i]), rsrc, at, 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b16(one_bf16(y[i]), rsrc, at, 0, 0);
+      }
+    }
+  }
+};
+
+// Sum over a wave in six vector adds whose second operand comes from another lane (no trip through LDS): neighbours,
+// pairs, halves of a row of 16 lanes, the row's mirror, then each row's last lane on to the next rows.  Lane 63 has
+// the total; it is read back as a scalar.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float bn_lane_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, true));
+}
+__device__ __forceinline__ float bn_wave_sum(float v) {
+  v = bn_lane_add<0xb1, 0xf>(v);   // quad_perm [1, 0, 3, 2]
+  v = bn_lane_add<0x4e, 0xf>(v);   // quad_perm [2, 3, 0, 1]
+  v = bn_lane_add<0x141, 0xf>(v);  // row_half_mirror
+  v = bn_lane_add<0x140, 0xf>(v);  // row_mirror
+  v = bn_lane_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+  v = bn_lane_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// A barrier that orders LDS only: loads of the next row stay in flight across it.
+__device__ __forceinline__ void bn_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // Sum over the threads of a row: one wave, or the whole workgroup through `slots` (16 floats).  Two calls in turn
@@ -77,20 +111,23 @@ __device__ __forceinline__ void bn_store(char* row, int v, int H, const float* y
 // every thread passes after its reads of the first.
 template <bool ONEWAVE>
 __device__ __forceinline__ float bn_row_sum(float v, float* slots) {
-  v = wave_sum(v);
+  v = bn_wave_sum(v);
   if (ONEWAVE) return v;
   const int wid = threadIdx.x >> 6, nw = blockDim.x >> 6;
   if ((threadIdx.x & 63) == 0) slots[wid] = v;
-  __syncthreads();
+  bn_barrier();
   float r = slots[0];
   for (int i = 1; i < nw; ++i) r += slots[i];
   return r;
 }
 
+// Floats from one partial row to the next: whole cache lines.
+__host__ __device__ __forceinline__ int64_t bn_part_pitch(int64_t H) { return (H + 31) / 32 * 32; }
+
 struct BnRows {  // base address and row pitch in bytes
   const char* p;
   int64_t pitch;
-  __device__ __forceinline__ const char* row(int64_t r) const { return p + r * pitch; }
+  __device__ __forceinline__ const char* row(int64_t r) const { return p ? p + r * pitch : nullptr; }
 };
 struct BnRowsOut {
   char* p;
@@ -103,286 +140,381 @@ __device__ __forceinline__ float bn_elem(const char* p) {
   return DT == PRL_F32 ? *reinterpret_cast<const float*>(p) : bf16_one(*reinterpret_cast<const uint16_t*>(p));
 }
 
-// ONEWAVE: a wave per row, blockDim / 64 rows at a time; otherwise a workgroup per row.
-template <int DT, int NV, bool ONEWAVE, bool AL>
-__global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_fwd(BnRows x, BnRows b, const char* __restrict__ w1,
-                                                          const char* __restrict__ w2, int gate_kind, BnRows gate,
-                                                          float scale, float offset, float eps1, float eps2,
-                                                          BnRowsOut h, BnRowsOut y, float* __restrict__ rstd1,
-                                                          float* __restrict__ rstd2, int64_t rows, int H) {
-  constexpr int VE = DT == PRL_F32 ? 4 : 8;
+// Places beyond a row's end read as 0 and add 0 to every sum: they are not masked.  (Only a factor that is not finite
+// makes them something else, and then the row's own values are not numbers either.)
+
+// Keeps a unit in its packed form through a loop: the compiler would unpack what does not change in front of it,
+// into twice the registers.
+__device__ __forceinline__ void bn_keep_packed(u32x4& v) { asm volatile("" : "+v"(v)); }
+
+// How the gate comes: not at all, as one value or one per row (GATE 0), one per channel (1, kept over the rows), one
+// per element (2).
+template <int NV, bool BWD, int GATE>
+struct BnRow {  // what a thread reads of one row, as it lies in memory
+  u32x4 x[NV], b[NV], gy[BWD ? NV : 1], gh[BWD ? NV : 1], g[GATE == 2 ? NV : 1];
+  float r1, r2, gt;
+};
+struct BnIn {
+  BnRows x, b, gy, gh, gate;
+  const float *rstd1, *rstd2;
+  const char *w1, *w2;
+  int gate_kind;
+};
+
+template <int DT, int NV, bool BWD, int GATE, bool VEC>
+__device__ __forceinline__ void bn_fetch(BnRow<NV, BWD, GATE>& r, const BnIn& in, int64_t row, int li, int tpr, int H) {
+  using U = BnUnit<DT, VEC>;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    r.b[k] = U::load(in.b.row(row), k, li, tpr, H);
+    r.x[k] = U::load(in.x.row(row), k, li, tpr, H);
+    if (BWD) r.gy[k] = U::load(in.gy.row(row), k, li, tpr, H);
+    if (BWD) r.gh[k] = U::load(in.gh.row(row), k, li, tpr, H);
+    if (GATE == 2) r.g[k] = U::load(in.gate.row(row), k, li, tpr, H);
+  }
+  r.r1 = BWD && in.rstd1 ? in.rstd1[row] : 1.0f;
+  r.r2 = BWD && in.rstd2 ? in.rstd2[row] : 0.0f;
+  r.gt = GATE == 0 && in.gate_kind != PRL_GATE_NONE ? bn_elem<DT>(in.gate.row(row)) : 1.0f;
+}
+
+// What a thread reads once: its columns of the weights and of a gate per channel.
+template <int DT, int NV, int GATE, bool VEC>
+struct BnCols {
+  using U = BnUnit<DT, VEC>;
+  u32x4 w1[NV], w2[NV], g[GATE ? NV : 1];
+  __device__ __forceinline__ void load(const BnIn& in, int li, int tpr, int H) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      w1[k] = U::load(in.w1, k, li, tpr, H);
+      w2[k] = U::load(in.w2, k, li, tpr, H);
+      if (GATE == 1) g[k] = U::load(in.gate.p, k, li, tpr, H);
+    }
+  }
+  // Keeps them packed through the loop over rows: the compiler would unpack what does not change in front of it, into
+  // twice the registers.
+  __device__ __forceinline__ void keep() {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      asm volatile("" : "+v"(w1[k]), "+v"(w2[k]));
+      if (GATE == 1) asm volatile("" : "+v"(g[GATE ? k : 0]));
+    }
+  }
+};
+
+// Places beyond a row's end read as 0 and add 0 to every sum: they are not masked.  (Only a factor that is not finite
+// makes them something else, and then the row's own values are not numbers either.)
+
+// ONEWAVE: a wave per row, blockDim / 64 rows at a time; otherwise a workgroup per row.  The next row's loads go out
+// as soon as this one's are unpacked and stay in flight while it is worked on.  BOTH: both weights are there.
+template <int DT, int NV, bool ONEWAVE, int GATE, bool VEC, bool BOTH>
+__global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_fwd(BnIn in, float scale, float offset, float eps1,
+                                                                          float eps2, BnRowsOut h, BnRowsOut y,
+                                                                          float* __restrict__ rstd1,
+                                                                          float* __restrict__ rstd2, int64_t rows, int H) {
+  using U = BnUnit<DT, VEC>;
+  constexpr int VE = U::kN;
+  const bool has1 = BOTH || in.w1 != nullptr, has2 = BOTH || in.w2 != nullptr;
   __shared__ float slots[2][16];
   const int tpr = ONEWAVE ? 64 : blockDim.x;
   const int li = ONEWAVE ? threadIdx.x & 63 : threadIdx.x;
-  const int rpb = ONEWAVE ? blockDim.x >> 6 : 1;
-  const int nvec = (H + VE - 1) / VE;
   const float inv_h = 1.0f / (float)H;
-  for (int64_t row = (int64_t)blockIdx.x * rpb + (ONEWAVE ? threadIdx.x >> 6 : 0); row < rows;
-       row += (int64_t)gridDim.x * rpb) {
-    float bv[NV][VE], hv[NV][VE];
+  const int64_t step = (int64_t)gridDim.x * (ONEWAVE ? blockDim.x >> 6 : 1);
+  int64_t row = (int64_t)blockIdx.x * (ONEWAVE ? blockDim.x >> 6 : 1) +
+                (ONEWAVE ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+  if (row >= rows) return;
+  BnCols<DT, NV, GATE, VEC> w;
+  BnRow<NV, false, GATE> cur;
+  bn_fetch<DT, NV, false, GATE, VEC>(cur, in, row, li, tpr, H);
+  w.load(in, li, tpr, H);
+  for (;;) {
+    const int64_t next = row + step;
+    w.keep();
+    float hv[NV][VE], bv[NV][VE];
     float ss = 0.0f;
+    if (GATE == 2) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) w.g[GATE ? k : 0] = cur.g[GATE == 2 ? k : 0];
+    }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int v = li + k * tpr;
-#pragma unroll
-      for (int i = 0; i < VE; ++i) bv[k][i] = hv[k][i] = 0.0f;
-      if (v < nvec) {
-        bn_load<DT, AL>(b.row(row), v, H, bv[k]);
-        bn_load<DT, AL>(x.row(row), v, H, hv[k]);
-      }
+      U::decode(cur.b[k], bv[k]);
+      U::decode(cur.x[k], hv[k]);
 #pragma unroll
       for (int i = 0; i < VE; ++i) ss = fmaf(bv[k][i], bv[k][i], ss);
     }
+    const float gt = cur.gt;
+    if (next < rows) bn_fetch<DT, NV, false, GATE, VEC>(cur, in, next, li, tpr, H);
     float r1 = 1.0f;
-    if (w1) {
+    if (has1) {
       r1 = rsqrtf(bn_row_sum<ONEWAVE>(ss, slots[0]) * inv_h + eps1);
       if (rstd1 && li == 0) rstd1[row] = r1;
     }
-    float gs = scale;
-    if (gate_kind == PRL_GATE_TOKEN || gate_kind == PRL_GATE_ONE) gs *= bn_elem<DT>(gate.row(row));
+    const float gs = scale * gt * r1;
     ss = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int v = li + k * tpr;
-      if (v < nvec) {
-        float f[VE];
+      float f[VE], t[VE];
 #pragma unroll
-        for (int i = 0; i < VE; ++i) f[i] = gs * r1;
-        if (w1) {
-          float w[VE];
-          bn_load<DT, AL>(w1, v, H, w);
+      for (int i = 0; i < VE; ++i) f[i] = gs;
+      if (has1) {
+        U::decode(w.w1[k], t);
 #pragma unroll
-          for (int i = 0; i < VE; ++i) f[i] *= w[i] + offset;
-        }
-        if (gate_kind == PRL_GATE_CHANNEL || gate_kind == PRL_GATE_FULL) {
-          float g[VE];
-          bn_load<DT, AL>(gate_kind == PRL_GATE_FULL ? gate.row(row) : gate.p, v, H, g);
+        for (int i = 0; i < VE; ++i) f[i] *= t[i] + offset;
+      }
+      if (GATE) {
+        U::decode(w.g[GATE ? k : 0], t);
 #pragma unroll
-          for (int i = 0; i < VE; ++i) f[i] *= g[i];
-        }
-#pragma unroll
-        for (int i = 0; i < VE; ++i) hv[k][i] = fmaf(f[i], bv[k][i], hv[k][i]);
-        bn_store<DT, AL>(h.row(row), v, H, hv[k]);
+        for (int i = 0; i < VE; ++i) f[i] *= t[i];
       }
 #pragma unroll
-      for (int i = 0; i < VE; ++i)
-        if (AL || v * VE + i < H) ss = fmaf(hv[k][i], hv[k][i], ss);
+      for (int i = 0; i < VE; ++i) {
+        hv[k][i] = fmaf(f[i], bv[k][i], hv[k][i]);
+        ss = fmaf(hv[k][i], hv[k][i], ss);
+      }
+      U::store(h.row(row), k, li, tpr, H, hv[k]);
     }
-    if (w2) {
+    if (has2) {
       const float r2 = rsqrtf(bn_row_sum<ONEWAVE>(ss, slots[1]) * inv_h + eps2);
       if (rstd2 && li == 0) rstd2[row] = r2;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int v = li + k * tpr;
-        if (v < nvec) {
-          float w[VE];
-          bn_load<DT, AL>(w2, v, H, w);
+        float t[VE];
+        U::decode(w.w2[k], t);
 #pragma unroll
-          for (int i = 0; i < VE; ++i) w[i] = (w[i] + offset) * (hv[k][i] * r2);
-          bn_store<DT, AL>(y.row(row), v, H, w);
-        }
+        for (int i = 0; i < VE; ++i) t[i] = (t[i] + offset) * (hv[k][i] * r2);
+        U::store(y.row(row), k, li, tpr, H, t);
       }
     }
-    if (!ONEWAVE && !(w1 && w2)) __syncthreads();  // one set of slots only: it is written again by the next row
+    if (next >= rows) break;
+    if (!ONEWAVE && !(has1 && has2)) bn_barrier();  // one set of slots only: it is written again by the next row
+    row = next;
   }
 }
 
 // part[array][blockIdx.x][H]: arrays 0 gw1, 1 gw2, 2 a channel gate's gradient (for a gate of one value: [blockIdx.x]),
 // each there only when asked for
-template <int DT, int NV, bool ONEWAVE, bool AL>
-__global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_bwd(
-    BnRows x, BnRows b, const char* __restrict__ w1, const char* __restrict__ w2, int gate_kind, BnRows gate, float scale,
-    float offset, const float* __restrict__ rstd1, const float* __restrict__ rstd2, BnRows gh, BnRows gy, BnRowsOut gx,
-    BnRowsOut gb, float* __restrict__ part1, float* __restrict__ part2, float* __restrict__ partg, BnRowsOut gg,
-    int64_t rows, int H) {
-  constexpr int VE = DT == PRL_F32 ? 4 : 8;
+template <int DT, int NV, bool ONEWAVE, int GATE, bool VEC, bool BOTH>
+__global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_bwd(BnIn in, float scale, float offset, BnRowsOut gx,
+                                                                          BnRowsOut gb, float* __restrict__ part1,
+                                                                          float* __restrict__ part2,
+                                                                          float* __restrict__ partg, BnRowsOut gg,
+                                                                          int64_t rows, int H) {
+  using U = BnUnit<DT, VEC>;
+  constexpr int VE = U::kN;
+  const bool has1 = BOTH || in.w1 != nullptr, has2 = BOTH || in.w2 != nullptr;
   __shared__ float slots[3][16];
   extern __shared__ float lds[];  // ONEWAVE: rows of the workgroup x H
   const int tpr = ONEWAVE ? 64 : blockDim.x;
   const int li = ONEWAVE ? threadIdx.x & 63 : threadIdx.x;
-  const int slot = ONEWAVE ? threadIdx.x >> 6 : 0;
+  const int slot = ONEWAVE ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const int rpb = ONEWAVE ? blockDim.x >> 6 : 1;
-  const int nvec = (H + VE - 1) / VE;
   const float inv_h = 1.0f / (float)H;
-  float a1[NV][VE], a2[NV][VE], ag[NV][VE], aone = 0.0f;
+  const int64_t step = (int64_t)gridDim.x * rpb;
+  float a1[NV][VE], a2[NV][VE], ag[GATE == 1 ? NV : 1][VE], aone = 0.0f;
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
-    for (int i = 0; i < VE; ++i) a1[k][i] = a2[k][i] = ag[k][i] = 0.0f;
-  for (int64_t row = (int64_t)blockIdx.x * rpb + slot; row < rows; row += (int64_t)gridDim.x * rpb) {
-    const float r1 = w1 ? rstd1[row] : 1.0f;
-    const float r2 = w2 ? rstd2[row] : 0.0f;
-    const float gt = gate_kind == PRL_GATE_TOKEN || gate_kind == PRL_GATE_ONE ? bn_elem<DT>(gate.row(row)) : 1.0f;
-    float bh[NV][VE], hh[NV][VE], G[NV][VE], q[NV][VE];  // q: gy (w2 + o), later u (w1 + o)
+    for (int i = 0; i < VE; ++i) a1[k][i] = a2[k][i] = ag[GATE == 1 ? k : 0][i] = 0.0f;
+  int64_t row = (int64_t)blockIdx.x * rpb + slot;
+  BnCols<DT, NV, GATE, VEC> w;
+  BnRow<NV, true, GATE> cur;
+  if (row < rows) bn_fetch<DT, NV, true, GATE, VEC>(cur, in, row, li, tpr, H);
+  w.load(in, li, tpr, H);
+  while (row < rows) {
+    const int64_t next = row + step;
+    w.keep();
+    const float r1 = cur.r1, r2 = cur.r2, gt = cur.gt;
+    float bh[NV][VE], hh[NV][VE], q[NV][VE];  // q: gy (w2 + o), then G, then G's share of the branch
+    u32x4 ghr[NV];
     float dot = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int v = li + k * tpr;
+      ghr[k] = cur.gh[k];
+      if (GATE == 2) w.g[GATE ? k : 0] = cur.g[GATE == 2 ? k : 0];
+      U::decode(cur.b[k], bh[k]);
 #pragma unroll
-      for (int i = 0; i < VE; ++i) bh[k][i] = hh[k][i] = G[k][i] = q[k][i] = 0.0f;
-      if (v < nvec) {
-        float t[VE], w[VE];
-        bn_load<DT, AL>(b.row(row), v, H, bh[k]);
-        if (w2) {
-          bn_load<DT, AL>(x.row(row), v, H, hh[k]);
-          bn_load<DT, AL>(gy.row(row), v, H, t);
+      for (int i = 0; i < VE; ++i) bh[k][i] *= r1;
+      if (has2) {
+        float f[VE], t[VE];
 #pragma unroll
-          for (int i = 0; i < VE; ++i) w[i] = scale * gt * r1;
-          if (w1) {
-            float z[VE];
-            bn_load<DT, AL>(w1, v, H, z);
+        for (int i = 0; i < VE; ++i) f[i] = scale * gt;
+        if (has1) {
+          U::decode(w.w1[k], t);
 #pragma unroll
-            for (int i = 0; i < VE; ++i) w[i] *= z[i] + offset;
-          }
-          if (gate_kind == PRL_GATE_CHANNEL || gate_kind == PRL_GATE_FULL) {
-            float z[VE];
-            bn_load<DT, AL>(gate_kind == PRL_GATE_FULL ? gate.row(row) : gate.p, v, H, z);
-#pragma unroll
-            for (int i = 0; i < VE; ++i) w[i] *= z[i];
-          }
-#pragma unroll
-          for (int i = 0; i < VE; ++i) hh[k][i] = fmaf(w[i], bh[k][i], hh[k][i]) * r2;
-          bn_load<DT, AL>(w2, v, H, w);
-#pragma unroll
-          for (int i = 0; i < VE; ++i) {
-            if (part2) a2[k][i] = fmaf(t[i], hh[k][i], a2[k][i]);
-            q[k][i] = t[i] * (w[i] + offset);
-            if (AL || v * VE + i < H) dot = fmaf(q[k][i], hh[k][i], dot);
-          }
+          for (int i = 0; i < VE; ++i) f[i] *= t[i] + offset;
         }
-        if (gh.p) bn_load<DT, AL>(gh.row(row), v, H, G[k]);
+        if (GATE) {
+          U::decode(w.g[GATE ? k : 0], t);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) bh[k][i] *= r1;
-      }
-    }
-    if (w2) {
-      dot = bn_row_sum<ONEWAVE>(dot, slots[0]) * inv_h;
-#pragma unroll
-      for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int i = 0; i < VE; ++i) G[k][i] = fmaf(r2, q[k][i] - hh[k][i] * dot, G[k][i]);
-    }
-    dot = 0.0f;
-    float gdot = 0.0f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int v = li + k * tpr;
-      if (v < nvec) {
-        float w[VE], g[VE];
-        bn_store<DT, AL>(gx.row(row), v, H, G[k]);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) w[i] = 1.0f, g[i] = gt;
-        if (w1) {
-          bn_load<DT, AL>(w1, v, H, w);
-#pragma unroll
-          for (int i = 0; i < VE; ++i) w[i] += offset;
+          for (int i = 0; i < VE; ++i) f[i] *= t[i];
         }
-        if (gate_kind == PRL_GATE_CHANNEL || gate_kind == PRL_GATE_FULL)
-          bn_load<DT, AL>(gate_kind == PRL_GATE_FULL ? gate.row(row) : gate.p, v, H, g);
+        U::decode(cur.x[k], hh[k]);
+        U::decode(cur.gy[k], t);
+        U::decode(w.w2[k], q[k]);
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
-          const bool in = AL || v * VE + i < H;
-          const float gn = scale * G[k][i] * bh[k][i] * w[i];  // the gate's gradient
-          const float u = scale * g[i] * G[k][i];
-          if (part1) a1[k][i] = fmaf(u, bh[k][i], a1[k][i]);
-          if (partg && gate_kind == PRL_GATE_CHANNEL) ag[k][i] += gn;
-          if (in) gdot += gn;
-          q[k][i] = u * w[i];
-          if (in) dot = fmaf(q[k][i], bh[k][i], dot);
-          w[i] = gn;
+          hh[k][i] = fmaf(f[i], bh[k][i], hh[k][i]) * r2;
+          q[k][i] = t[i] * (q[k][i] + offset);
+          a2[k][i] = fmaf(t[i], hh[k][i], a2[k][i]);
+          dot = fmaf(q[k][i], hh[k][i], dot);
         }
-        if (gate_kind == PRL_GATE_FULL && gg.p) bn_store<DT, AL>(gg.row(row), v, H, w);
       }
     }
-    aone += gdot;
-    if (gate_kind == PRL_GATE_TOKEN && gg.p) {
-      gdot = bn_row_sum<ONEWAVE>(gdot, slots[2]);
-      if (li == 0) store_elem<DT>(gg.row(row), 0, gdot);
-    }
-    dot = w1 ? bn_row_sum<ONEWAVE>(dot, slots[1]) * inv_h : 0.0f;
+    if (next < rows) bn_fetch<DT, NV, true, GATE, VEC>(cur, in, next, li, tpr, H);
+    if (has2) dot = bn_row_sum<ONEWAVE>(dot, slots[0]) * inv_h;
+    float dot1 = 0.0f, gdot = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int v = li + k * tpr;
-      if (v < nvec) {
+      float t[VE], v[VE];
+      U::decode(ghr[k], t);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) q[k][i] = r1 * (q[k][i] - bh[k][i] * dot);
-        bn_store<DT, AL>(gb.row(row), v, H, q[k]);
+      for (int i = 0; i < VE; ++i) q[k][i] = has2 ? fmaf(r2, q[k][i] - hh[k][i] * dot, t[i]) : t[i];
+      U::store(gx.row(row), k, li, tpr, H, q[k]);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) v[i] = 1.0f, t[i] = gt;
+      if (has1) {
+        U::decode(w.w1[k], v);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) v[i] += offset;
+      }
+      if (GATE) U::decode(w.g[GATE ? k : 0], t);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        const float s = scale * q[k][i];
+        const float gn = s * bh[k][i] * v[i];  // the gate's gradient
+        const float u = s * t[i];
+        q[k][i] = u * v[i];
+        a1[k][i] = fmaf(u, bh[k][i], a1[k][i]);
+        if (GATE == 0) gdot += gn;
+        if (GATE == 1) ag[GATE == 1 ? k : 0][i] += gn;
+        dot1 = fmaf(q[k][i], bh[k][i], dot1);
+        v[i] = gn;
+      }
+      if (GATE == 2 && gg.p) U::store(gg.row(row), k, li, tpr, H, v);
+    }
+    if (GATE == 0) {
+      aone += gdot;
+      if (gg.p) {
+        gdot = bn_row_sum<ONEWAVE>(gdot, slots[2]);
+        if (li == 0) store_elem<DT>(gg.row(row), 0, gdot);
       }
     }
-    if (!ONEWAVE) __syncthreads();  // slots are written again by the next row
+    if (has1) dot1 = bn_row_sum<ONEWAVE>(dot1, slots[1]) * inv_h;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) q[k][i] = has1 ? r1 * (q[k][i] - bh[k][i] * dot1) : q[k][i];
+      U::store(gb.row(row), k, li, tpr, H, q[k]);
+    }
+    if (!ONEWAVE && !(has1 && has2)) bn_barrier();  // a set of slots would be written again with no barrier between
+    row = next;
   }
-  if (gate_kind == PRL_GATE_ONE && partg) {
+  if (GATE == 0 && partg) {
     __syncthreads();
     aone = bn_row_sum<false>(aone, slots[2]);
     if (threadIdx.x == 0) partg[blockIdx.x] = aone;
   }
-  float* const part[3] = {part1, part2, gate_kind == PRL_GATE_ONE ? nullptr : partg};
+  float* const part[3] = {part1, part2, GATE == 1 ? partg : nullptr};
 #pragma unroll
-  for (int a = 0; a < 3; ++a) {
+  for (int a = 0; a < (GATE == 1 ? 3 : 2); ++a) {
     if (!part[a]) continue;
-    float(&acc)[NV][VE] = a == 0 ? a1 : a == 1 ? a2 : ag;
-    float* out = part[a] + (int64_t)blockIdx.x * H;
+    float* out = part[a] + (int64_t)blockIdx.x * bn_part_pitch(H);
     if (ONEWAVE) __syncthreads();
+    float* mine = ONEWAVE ? lds + slot * bn_part_pitch(H) : out;
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) {
+      const float* z = a == 0 ? a1[k] : a == 1 ? a2[k] : ag[GATE == 1 ? k : 0];
 #pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        const int c = (li + k * tpr) * VE + i;
-        if (c < H) (ONEWAVE ? lds + slot * H : out)[c] = acc[k][i];
+      for (int i = 0; i < VE; i += VEC ? 4 : 1) {
+        const int c = U::column(k, i, li, tpr);
+        if (c >= H) continue;
+        if (VEC) *reinterpret_cast<float4*>(mine + c) = make_float4(z[i], z[i + 1], z[i + 2], z[i + 3]);
+        else mine[c] = z[i];
       }
+    }
     if (ONEWAVE) {
       __syncthreads();
       for (int c = threadIdx.x; c < H; c += blockDim.x) {
         float s = lds[c];
-        for (int r = 1; r < rpb; ++r) s += lds[r * H + c];
+        for (int r = 1; r < rpb; ++r) s += lds[r * bn_part_pitch(H) + c];
         out[c] = s;
       }
     }
   }
 }
 
-// out[a][c] = sum over the partial rows of part[a][p][c], in a fixed order; 32 columns a workgroup, 32 groups of
-// threads over the rows.
+// out[a][c] = sum over the partial rows of part[a][p][c], in a fixed order.  A workgroup owns 32 columns (whole cache
+// lines); 32 groups of 8 threads take every 32nd row, four columns a thread, eight rows in flight.
 template <int DT>
-__global__ __launch_bounds__(1024) void k_block_norms_finish(const float* p0, const float* p1, const float* p2, char* o0,
-                                                             char* o1, char* o2, int nparts, int H, int Hg) {
+__global__ __launch_bounds__(256) void k_block_norms_finish(const float* p0, const float* p1, const float* p2, char* o0,
+                                                            char* o1, char* o2, int nparts, int H, int gate_one) {
   const float* part = blockIdx.y == 0 ? p0 : blockIdx.y == 1 ? p1 : p2;
   char* out = blockIdx.y == 0 ? o0 : blockIdx.y == 1 ? o1 : o2;
-  if (blockIdx.y == 2) H = Hg;  // a gate of one value has one column
-  if (!part || (int)blockIdx.x * 32 >= H) return;
+  if (!part) return;
   __shared__ float lds[32][33];
-  const int lc = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lc;
-  float s = 0.0f;
-  if (c < H)
-    for (int p = g; p < nparts; p += 32) s += part[(int64_t)p * H + c];
-  lds[g][lc] = s;
-  __syncthreads();
-  if (g == 0 && c < H) {
-    float t = lds[0][lc];
+  if (gate_one && blockIdx.y == 2) {  // one value from every workgroup
+    if (blockIdx.x) return;
+    float s = 0.0f;
+    for (int i = threadIdx.x; i < nparts; i += 256) s += part[i];
+    s = block_sum<4>(s, lds[0]);
+    if (threadIdx.x == 0) store_elem<DT>(out, 0, s);
+    return;
+  }
+  const int q = threadIdx.x & 7, g = threadIdx.x >> 3;
+  const int64_t pitch = bn_part_pitch(H) / 4;
+  const float4* at = reinterpret_cast<const float4*>(part) + blockIdx.x * 8 + q;
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int p = g; p < nparts; p += 256) {
+    float4 z[8];
 #pragma unroll
-    for (int k = 1; k < 32; ++k) t += lds[k][lc];
+    for (int j = 0; j < 8; ++j) z[j] = p + 32 * j < nparts ? at[(p + 32 * j) * pitch] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s.x += z[j].x, s.y += z[j].y, s.z += z[j].z, s.w += z[j].w;
+  }
+  lds[g][4 * q] = s.x, lds[g][4 * q + 1] = s.y, lds[g][4 * q + 2] = s.z, lds[g][4 * q + 3] = s.w;
+  __syncthreads();
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  if (threadIdx.x < 32 && c < H) {
+    float t = lds[0][threadIdx.x];
+#pragma unroll
+    for (int k = 1; k < 32; ++k) t += lds[k][threadIdx.x];
     store_elem<DT>(out, c, t);
   }
 }
 
 // Threads of a row and units a thread: one wave while a row has at most 128 units, else as many waves as give each
-// thread one unit of bf16 or two of fp32 (8 elements).
+// thread one unit (two where that would be over 16 waves).
 struct BnShape {
   bool onewave;
   int nv, threads, rpb;
 };
-static BnShape bn_shape(int dtype, int64_t H) {
-  const int ve = dtype == PRL_F32 ? 4 : 8;
-  const int64_t nvec = (H + ve - 1) / ve;
-  if (nvec <= 64) return {true, 1, 256, 4};
-  if (nvec <= 128) return {true, 2, 256, 4};
-  const int nv = dtype == PRL_F32 ? 2 : 1;
-  return {false, nv, (int)(((nvec + nv - 1) / nv + 63) / 64 * 64), 1};
+static BnShape bn_shape(int dtype, int64_t H, bool vec) {
+  const int n = !vec || dtype == PRL_F32 ? 4 : 8;
+  const int64_t units = (H + n - 1) / n;
+  if (units <= 64) return {true, 1, 256, 4};
+  if (units <= 128) return {true, 2, 256, 4};
+  const int nv = units > 1024 ? 2 : 1;
+  return {false, nv, (int)(((units + nv - 1) / nv + 63) / 64 * 64), 1};
 }
 static int bn_blocks(int64_t rows, int rpb, int cap) {
   const int64_t want = (rows + rpb - 1) / rpb;
   return (int)(want < cap ? (want > 0 ? want : 1) : cap);
+}
+
+// Forward: one row per wave or workgroup and as many workgroups as there are rows, except for the widest rows (7 waves
+// and more), where few workgroups that fetch the next row while they wait for this one's sums are ahead (8192 rows of
+// 5120 bf16: 65.1 us with 256 workgroups, 75 with one per row; 16384 rows of 2048: 48.5 us with one per row, 54 with
+// 1024).
+static int bn_fwd_blocks(int64_t rows, const BnShape& sh) {
+  const int waves = sh.threads / 64;
+  return bn_blocks(rows, sh.rpb, sh.onewave || waves < 7 ? 1 << 20 : 256 * (waves < 16 ? 16 / waves : 1));
+}
+// Backward: every workgroup leaves a partial row per weight, so as few as keep 8 waves on each compute unit (16 where
+// the accesses are single elements): 8192 rows of 5120 bf16 101 us with 256, 122 with 512; 16384 rows of 2048 84 us with
+// 512, 106 with 256.
+static int bn_bwd_blocks(int64_t rows, const BnShape& sh, bool vec) {
+  const int waves = sh.threads / 64, want = vec ? 8 : 16;
+  return bn_blocks(rows, sh.rpb, 256 * (want > waves ? want / waves : 1));
 }
 
 }  // namespace prl
@@ -395,7 +527,8 @@ extern "C" int prl_block_norms_supported(int dtype, int64_t H) {
 
 extern "C" size_t prl_block_norms_bwd_workspace_bytes(int dtype, int64_t rows, int64_t H) {
   if (!prl_block_norms_supported(dtype, H) || rows < 0) return 0;
-  return (size_t)3 * bn_blocks(rows, bn_shape(dtype, H).rpb, kBnMaxBlocks) * (size_t)H * sizeof(float);
+  const int a = bn_bwd_blocks(rows, bn_shape(dtype, H, true), true), b = bn_bwd_blocks(rows, bn_shape(dtype, H, false), false);
+  return (size_t)3 * (a > b ? a : b) * bn_part_pitch(H) * sizeof(float);
 }
 
 static bool bn_aligned(int es, int64_t H, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides) {
@@ -419,17 +552,33 @@ static int bn_check(const char* who, int dtype, int64_t rows, int64_t H, int gat
   return PRL_OK;
 }
 
-#define PRL_BN_DISPATCH(KERNEL)                                                   \
-  do {                                                                            \
-    if (dtype == PRL_BF16) {                                                      \
-      if (!sh.onewave) { if (al) KERNEL(PRL_BF16, 1, false, true); else KERNEL(PRL_BF16, 1, false, false); }   \
-      else if (sh.nv == 1) { if (al) KERNEL(PRL_BF16, 1, true, true); else KERNEL(PRL_BF16, 1, true, false); } \
-      else { if (al) KERNEL(PRL_BF16, 2, true, true); else KERNEL(PRL_BF16, 2, true, false); }                 \
-    } else {                                                                      \
-      if (!sh.onewave) { if (al) KERNEL(PRL_F32, 2, false, true); else KERNEL(PRL_F32, 2, false, false); }     \
-      else if (sh.nv == 1) { if (al) KERNEL(PRL_F32, 1, true, true); else KERNEL(PRL_F32, 1, true, false); }   \
-      else { if (al) KERNEL(PRL_F32, 2, true, true); else KERNEL(PRL_F32, 2, true, false); }                   \
-    }                                                                             \
+#define PRL_BN_GATE(KERNEL, DT, NV, OW, VEC, BOTH)                                      \
+  do {                                                                                  \
+    if (gate_kind == PRL_GATE_FULL) KERNEL(DT, NV, OW, 2, VEC, BOTH);                   \
+    else if (gate_kind == PRL_GATE_CHANNEL) KERNEL(DT, NV, OW, 1, VEC, BOTH);           \
+    else KERNEL(DT, NV, OW, 0, VEC, BOTH);                                              \
+  } while (0)
+#define PRL_BN_VEC(KERNEL, DT, NV, OW, VEC)                            \
+  do {                                                                 \
+    if (w_post && w_pre) PRL_BN_GATE(KERNEL, DT, NV, OW, VEC, true);   \
+    else PRL_BN_GATE(KERNEL, DT, NV, OW, VEC, false);                  \
+  } while (0)
+#define PRL_BN_SHAPE(KERNEL, DT, VEC)                                   \
+  do {                                                                  \
+    if (sh.onewave && sh.nv == 1) PRL_BN_VEC(KERNEL, DT, 1, true, VEC); \
+    else if (sh.onewave) PRL_BN_VEC(KERNEL, DT, 2, true, VEC);          \
+    else PRL_BN_VEC(KERNEL, DT, 1, false, VEC);                         \
+  } while (0)
+#define PRL_BN_DISPATCH(KERNEL)                                                           \
+  do { /* (two units a thread of a workgroup: rows of more than 4096 fp32 or single elements) */ \
+    const bool wide = !sh.onewave && sh.nv == 2;                                          \
+    if (dtype == PRL_F32 && vec && wide) PRL_BN_VEC(KERNEL, PRL_F32, 2, false, true);     \
+    else if (dtype == PRL_F32 && vec) PRL_BN_SHAPE(KERNEL, PRL_F32, true);                \
+    else if (dtype == PRL_F32 && wide) PRL_BN_VEC(KERNEL, PRL_F32, 2, false, false);      \
+    else if (dtype == PRL_F32) PRL_BN_SHAPE(KERNEL, PRL_F32, false);                      \
+    else if (vec) PRL_BN_SHAPE(KERNEL, PRL_BF16, true);                                   \
+    else if (wide) PRL_BN_VEC(KERNEL, PRL_BF16, 2, false, false);                         \
+    else PRL_BN_SHAPE(KERNEL, PRL_BF16, false);                                           \
   } while (0)
 
 extern "C" int prl_block_norms_fwd(const void* x, int64_t x_stride, const void* branch, int64_t branch_stride,
@@ -448,18 +597,19 @@ extern "C" int prl_block_norms_fwd(const void* x, int64_t x_stride, const void* 
   const int64_t es = dtype == PRL_F32 ? 4 : 2;
   const bool narrow = gate_kind == PRL_GATE_TOKEN || gate_kind == PRL_GATE_ONE;
   const int64_t gate_pitch = gate_kind == PRL_GATE_ONE ? 0 : gate_stride * es;
-  const bool al = bn_aligned((int)es, H, {x, branch, w_post, w_pre, hidden, w_pre ? normed : nullptr,
+  const bool vec = bn_aligned((int)es, H, {x, branch, w_post, w_pre, hidden, w_pre ? normed : nullptr,
                                           narrow ? nullptr : gate},
                              {x_stride, branch_stride, hidden_stride, n_stride,
                               gate_kind == PRL_GATE_FULL ? gate_stride : 0});
-  const BnShape sh = bn_shape(dtype, H);
-  const dim3 grid((unsigned)bn_blocks(rows, sh.rpb, 1 << 20)), block((unsigned)sh.threads);
-#define PRL_BN_FWD(DT, NV, OW, AL)                                                                                   \
-  hipLaunchKernelGGL((k_block_norms_fwd<DT, NV, OW, AL>), grid, block, 0, (hipStream_t)stream,                       \
-                     (BnRows{(const char*)x, x_stride * es}), (BnRows{(const char*)branch, branch_stride * es}),      \
-                     (const char*)w_post, (const char*)w_pre, gate_kind, (BnRows{(const char*)gate, gate_pitch}), \
-                     scale, weight_offset, eps_post, eps_pre, (BnRowsOut{(char*)hidden, hidden_stride * es}),         \
-                     (BnRowsOut{(char*)normed, n_stride * es}), rstd_post, rstd_pre, rows, (int)H)
+  const BnShape sh = bn_shape(dtype, H, vec);
+  const dim3 grid((unsigned)bn_fwd_blocks(rows, sh)), block((unsigned)sh.threads);
+  const BnIn in = {{(const char*)x, x_stride * es}, {(const char*)branch, branch_stride * es}, {nullptr, 0}, {nullptr, 0},
+                   {(const char*)gate, gate_pitch}, nullptr, nullptr, (const char*)w_post, (const char*)w_pre, gate_kind};
+#define PRL_BN_FWD(DT, NV, OW, GATE, VEC, BOTH)                                                                       \
+  hipLaunchKernelGGL((k_block_norms_fwd<DT, NV, OW, GATE, VEC, BOTH>), grid, block, 0, (hipStream_t)stream, in, scale, \
+                     weight_offset, eps_post, eps_pre, (BnRowsOut{(char*)hidden, hidden_stride * es}),                \
+                     (BnRowsOut{(char*)normed, n_stride * es}), w_post ? rstd_post : nullptr,                         \
+                     w_pre ? rstd_pre : nullptr, rows, (int)H)
   PRL_BN_DISPATCH(PRL_BN_FWD);
 #undef PRL_BN_FWD
   PRL_CHECK_LAUNCH("block_norms_fwd");
@@ -488,47 +638,53 @@ extern "C" int prl_block_norms_bwd(const void* x, int64_t x_stride, const void* 
                             (!w_pre == !g_normed)),
               "block_norms_bwd: x, branch, gx, g_branch and (with their weights) rstd_post, rstd_pre, g_normed must not be "
               "NULL; g_normed goes with w_pre");
-  const BnShape sh = bn_shape(dtype, H);
-  const int nblk = bn_blocks(rows, sh.rpb, kBnMaxBlocks);
-  const size_t one = (size_t)nblk * H, need = 3 * one * sizeof(float);
+  const int64_t es = dtype == PRL_F32 ? 4 : 2;
+  const bool full = gate_kind == PRL_GATE_FULL, narrow = gate_kind == PRL_GATE_TOKEN || gate_kind == PRL_GATE_ONE;
+  const bool vec = bn_aligned((int)es, H,
+                             {x, branch, w_post, w_pre, g_hidden, g_normed, gx, g_branch,
+                              narrow ? nullptr : gate, full ? g_gate : nullptr},
+                             {x_stride, branch_stride, g_hidden ? g_hidden_stride : 0, g_normed ? g_normed_stride : 0,
+                              gx_stride, g_branch_stride, full ? gate_stride : 0, full && g_gate ? g_gate_stride : 0});
+  const BnShape sh = bn_shape(dtype, H, vec);
+  const int nblk = bn_bwd_blocks(rows, sh, vec);
+  const size_t one = (size_t)nblk * bn_part_pitch(H), need = 3 * one * sizeof(float);
   const bool channel = (gate_kind == PRL_GATE_CHANNEL || gate_kind == PRL_GATE_ONE) && g_gate;
   const bool sums = g_w_post || g_w_pre || channel;
   PRL_REQUIRE(!sums || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
               "block_norms_bwd: 16-byte aligned workspace of %zu bytes needed (prl_block_norms_bwd_workspace_bytes)", need);
   float* ws = (float*)workspace;
   float *p1 = g_w_post ? ws : nullptr, *p2 = g_w_pre ? ws + one : nullptr, *pg = channel ? ws + 2 * one : nullptr;
-  const int64_t es = dtype == PRL_F32 ? 4 : 2;
   hipStream_t st = (hipStream_t)stream;
   // rows == 0: the kernel runs with no row and leaves sums of zero
-  const bool full = gate_kind == PRL_GATE_FULL, narrow = gate_kind == PRL_GATE_TOKEN || gate_kind == PRL_GATE_ONE;
-  const bool al = bn_aligned((int)es, H,
-                             {x, branch, w_post, w_pre, g_hidden, g_normed, gx, g_branch,
-                              narrow ? nullptr : gate, full ? g_gate : nullptr},
-                             {x_stride, branch_stride, g_hidden ? g_hidden_stride : 0, g_normed ? g_normed_stride : 0,
-                              gx_stride, g_branch_stride, full ? gate_stride : 0, full && g_gate ? g_gate_stride : 0});
   const int64_t gate_pitch = gate_kind == PRL_GATE_ONE ? 0 : gate_stride * es;
   const dim3 grid((unsigned)nblk), block((unsigned)sh.threads);
-  const size_t lds = sh.onewave ? (size_t)sh.rpb * H * sizeof(float) : 0;
+  const size_t lds = sh.onewave ? (size_t)sh.rpb * bn_part_pitch(H) * sizeof(float) : 0;
   char* gg = channel || !g_gate ? nullptr : (char*)g_gate;
-#define PRL_BN_BWD(DT, NV, OW, AL)                                                                                    \
-  hipLaunchKernelGGL((k_block_norms_bwd<DT, NV, OW, AL>), grid, block, lds, st, (BnRows{(const char*)x, x_stride * es}), \
-                     (BnRows{(const char*)branch, branch_stride * es}), (const char*)w_post, (const char*)w_pre, gate_kind, \
-                     (BnRows{(const char*)gate, gate_pitch}), scale, weight_offset, rstd_post, rstd_pre,         \
-                     (BnRows{(const char*)g_hidden, g_hidden_stride * es}),                                           \
-                     (BnRows{(const char*)g_normed, g_normed_stride * es}), (BnRowsOut{(char*)gx, gx_stride * es}),    \
-                     (BnRowsOut{(char*)g_branch, g_branch_stride * es}), p1, p2, pg, (BnRowsOut{gg, g_gate_stride * es}), \
-                     rows, (int)H)
+  const BnIn in = {{(const char*)x, x_stride * es},
+                   {(const char*)branch, branch_stride * es},
+                   {(const char*)g_normed, g_normed_stride * es},
+                   {(const char*)g_hidden, g_hidden_stride * es},
+                   {(const char*)gate, gate_pitch},
+                   w_post ? rstd_post : nullptr,
+                   w_pre ? rstd_pre : nullptr,
+                   (const char*)w_post,
+                   (const char*)w_pre,
+                   gate_kind};
+#define PRL_BN_BWD(DT, NV, OW, GATE, VEC, BOTH)                                                                       \
+  hipLaunchKernelGGL((k_block_norms_bwd<DT, NV, OW, GATE, VEC, BOTH>), grid, block, lds, st, in, scale, weight_offset, \
+                     (BnRowsOut{(char*)gx, gx_stride * es}), (BnRowsOut{(char*)g_branch, g_branch_stride * es}), p1, p2, \
+                     pg, (BnRowsOut{gg, g_gate_stride * es}), rows, (int)H)
   PRL_BN_DISPATCH(PRL_BN_BWD);
 #undef PRL_BN_BWD
   PRL_CHECK_LAUNCH("block_norms_bwd");
   if (!sums) return PRL_OK;
   const dim3 fgrid((unsigned)((H + 31) / 32), 3);
   if (dtype == PRL_BF16)
-    hipLaunchKernelGGL((k_block_norms_finish<PRL_BF16>), fgrid, dim3(1024), 0, st, p1, p2, pg, (char*)g_w_post,
-                       (char*)g_w_pre, (char*)g_gate, nblk, (int)H, gate_kind == PRL_GATE_ONE ? 1 : (int)H);
+    hipLaunchKernelGGL((k_block_norms_finish<PRL_BF16>), fgrid, dim3(256), 0, st, p1, p2, pg, (char*)g_w_post,
+                       (char*)g_w_pre, (char*)g_gate, nblk, (int)H, gate_kind == PRL_GATE_ONE);
   else
-    hipLaunchKernelGGL((k_block_norms_finish<PRL_F32>), fgrid, dim3(1024), 0, st, p1, p2, pg, (char*)g_w_post,
-                       (char*)g_w_pre, (char*)g_gate, nblk, (int)H, gate_kind == PRL_GATE_ONE ? 1 : (int)H);
+    hipLaunchKernelGGL((k_block_norms_finish<PRL_F32>), fgrid, dim3(256), 0, st, p1, p2, pg, (char*)g_w_post,
+                       (char*)g_w_pre, (char*)g_gate, nblk, (int)H, gate_kind == PRL_GATE_ONE);
   PRL_CHECK_LAUNCH("block_norms_bwd");
   return PRL_OK;
 }

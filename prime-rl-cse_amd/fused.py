@@ -26,6 +26,17 @@ from . import _capi as C
 from . import lm_head
 
 
+def _first_derivative(backward: Any) -> Any:
+    """torch's `once_differentiable` for a backward that only launches kernels, at its cost (4 us of host time a call)
+    only where a graph of the backward is asked for: there a second derivative fails instead of being left out."""
+    once = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return once(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
+
+
 def _row_layout(x: Tensor):
     """How the kernels walk the rows of x (last dimension contiguous): (rows, row stride, group, group stride),
     group = 0 for evenly pitched rows, or None when x is neither that nor groups of evenly pitched rows."""
@@ -223,6 +234,21 @@ def _gate_rows(gate: Tensor, lead: tuple[int, ...], h: int) -> tuple[int, Tensor
                      f"{(*lead, 1)} or {(*lead, h)} (expand others yourself)")
 
 
+def _launch_block_norms(x: Tensor, branch: Tensor, w_post: Tensor | None, w_pre: Tensor | None, gate: Tensor | None,
+                        kind: int, scale: float, offset: float, eps_post: float, eps_pre: float, hidden: Tensor,
+                        normed: Tensor | None, rstd: Tensor | None) -> None:
+    dev = x.device
+    rows, h = x.shape
+    r1 = None if rstd is None else rstd.data_ptr()
+    with C.on_device(dev), C.timed("prl_block_norms_fwd", dev):
+        C.check(C.load().prl_block_norms_fwd(
+            x.data_ptr(), x.stride(0), branch.data_ptr(), branch.stride(0),
+            None if w_post is None else w_post.data_ptr(), None if w_pre is None else w_pre.data_ptr(), kind,
+            None if gate is None else gate.data_ptr(), 0 if gate is None else gate.stride(0), scale, offset, eps_post,
+            eps_pre, hidden.data_ptr(), h, None if normed is None else normed.data_ptr(), h, r1,
+            None if r1 is None else r1 + 4 * rows, C.dtype_code(x), rows, h, C.stream_ptr(dev)), "prl_block_norms_fwd")
+
+
 class _BlockNorms(torch.autograd.Function):
     """x, branch [rows, h] and the gate in one of its three layouts; see `block_norms`."""
 
@@ -231,52 +257,48 @@ class _BlockNorms(torch.autograd.Function):
                 kind: int, scale: float, offset: float, eps_post: float, eps_pre: float):
         dev = x.device
         rows, h = x.shape
-        train = any(ctx.needs_input_grad)
         hidden = torch.empty((rows, h), dtype=x.dtype, device=dev)
         normed = None if w_pre is None else torch.empty((rows, h), dtype=x.dtype, device=dev)
-        r1 = torch.empty(rows, dtype=torch.float32, device=dev) if train and w_post is not None else None
-        r2 = torch.empty(rows, dtype=torch.float32, device=dev) if train and w_pre is not None else None
-        with C.on_device(dev), C.timed("prl_block_norms_fwd", dev):
-            C.check(C.load().prl_block_norms_fwd(
-                C.ptr(x), x.stride(0), C.ptr(branch), branch.stride(0), C.ptr(w_post), C.ptr(w_pre), kind, C.ptr(gate),
-                0 if gate is None else gate.stride(0), scale, offset, eps_post, eps_pre, C.ptr(hidden), h,
-                C.ptr(normed), h, C.ptr(r1), C.ptr(r2), C.dtype_code(x), rows, h, C.stream_ptr(dev)),
-                "prl_block_norms_fwd")
-        ctx.save_for_backward(x, branch, w_post, w_pre, gate, r1, r2)
+        rstd = torch.empty(2 * rows, dtype=torch.float32, device=dev)  # of the branch, then of the sum
+        _launch_block_norms(x, branch, w_post, w_pre, gate, kind, scale, offset, eps_post, eps_pre, hidden, normed, rstd)
+        ctx.save_for_backward(x, branch, w_post, w_pre, gate, rstd)
         ctx.args = (kind, scale, offset)
         ctx.set_materialize_grads(False)
         return hidden, normed
 
     @staticmethod
-    @once_differentiable
+    @_first_derivative
     def backward(ctx, gh: Tensor | None, gy: Tensor | None):
-        x, branch, w_post, w_pre, gate, r1, r2 = ctx.saved_tensors
-        kind, scale, offset = ctx.args
         if gh is None and gy is None:
             return (None,) * 10
-        dev = x.device
+        x, branch, w_post, w_pre, gate, rstd = ctx.saved_tensors
+        kind, scale, offset = ctx.args
+        dev, dtype = x.device, x.dtype
         lib = C.load()
         rows, h = x.shape
         if gy is None:  # the normalised output went nowhere
-            w_pre = r2 = None
+            w_pre = None
         gh = None if gh is None else _pitched(gh, h)
         gy = None if gy is None else _pitched(gy, h)
         need = ctx.needs_input_grad
-        gx, gb = torch.empty((rows, h), dtype=x.dtype, device=dev), torch.empty((rows, h), dtype=x.dtype, device=dev)
+        gx, gb = torch.empty((rows, h), dtype=dtype, device=dev), torch.empty((rows, h), dtype=dtype, device=dev)
         g1 = torch.empty_like(w_post) if w_post is not None and need[2] else None
         g2 = torch.empty_like(w_pre) if w_pre is not None and need[3] else None
-        gg = torch.empty(gate.shape, dtype=x.dtype, device=dev) if gate is not None and need[4] else None
+        gg = torch.empty(gate.shape, dtype=dtype, device=dev) if gate is not None and need[4] else None
         code = C.dtype_code(x)
-        ws = None
+        ws, ws_bytes = None, 0
         if g1 is not None or g2 is not None or (gg is not None and kind in (C.GATE_CHANNEL, C.GATE_ONE)):
-            ws = torch.empty(lib.prl_block_norms_bwd_workspace_bytes(code, rows, h), dtype=torch.uint8, device=dev)
+            ws_bytes = lib.prl_block_norms_bwd_workspace_bytes(code, rows, h)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        at = lambda t: None if t is None else t.data_ptr()
+        pitch = lambda t: 0 if t is None else t.stride(0)
+        r1 = rstd.data_ptr()
         with C.on_device(dev), C.timed("prl_block_norms_bwd", dev):
             C.check(lib.prl_block_norms_bwd(
-                C.ptr(x), x.stride(0), C.ptr(branch), branch.stride(0), C.ptr(w_post), C.ptr(w_pre), kind, C.ptr(gate),
-                0 if gate is None else gate.stride(0), scale, offset, C.ptr(r1), C.ptr(r2), C.ptr(gh),
-                0 if gh is None else gh.stride(0), C.ptr(gy), 0 if gy is None else gy.stride(0), C.ptr(gx), h, C.ptr(gb),
-                h, C.ptr(g1), C.ptr(g2), C.ptr(gg), 0 if gg is None else gg.stride(0), code, rows, h, C.ptr(ws),
-                0 if ws is None else ws.numel(), C.stream_ptr(dev)), "prl_block_norms_bwd")
+                x.data_ptr(), x.stride(0), branch.data_ptr(), branch.stride(0), at(w_post), at(w_pre), kind, at(gate),
+                pitch(gate), scale, offset, r1, r1 + 4 * rows, at(gh), pitch(gh), at(gy), pitch(gy), gx.data_ptr(), h,
+                gb.data_ptr(), h, at(g1), at(g2), at(gg), pitch(gg), code, rows, h, at(ws), ws_bytes,
+                C.stream_ptr(dev)), "prl_block_norms_bwd")
         return gx, gb, g1, g2, gg, None, None, None, None, None
 
 
@@ -304,21 +326,31 @@ def block_norms(x: Tensor, branch: Tensor, post_weight: Tensor | None = None, pr
     without `pre_weight` normed is None.  `gate` is one value, one per channel [H], per row [..., 1] or per element
     (x's shape).  `pre_eps` defaults to `eps`.  fp32 inside, each output rounded once; `normed` is
     formed from the unrounded hidden (`add_rms_norm` rounds the sum first, as separate modules do)."""
-    dev = C.require_device(x, branch, post_weight, pre_weight, gate)
     if not block_norms_supported(x, branch, post_weight, pre_weight, gate):
+        dev = C.require_device(x, branch, post_weight, pre_weight, gate)
         raise ValueError("block_norms: x and branch of one shape with rows of 1 to 8192, weights of a row's length, all "
                          f"in one dtype (bf16 or fp32); got x {tuple(x.shape)} {x.dtype}, branch {tuple(branch.shape)} "
                          f"{branch.dtype}, weights " + ", ".join("none" if w is None else f"{tuple(w.shape)} {w.dtype}"
                                                                  for w in (post_weight, pre_weight)) + " on " + str(dev))
-    h, lead = x.shape[-1], tuple(x.shape[:-1])
+    shape = x.shape
+    h = shape[-1]
     kind = C.GATE_NONE
     if gate is not None:
-        kind, gate = _gate_rows(gate, lead, h)
+        kind, gate = _gate_rows(gate, tuple(shape[:-1]), h)
+    x, branch = _pitched(x, h), _pitched(branch, h)
     w1 = None if post_weight is None else post_weight.contiguous()
     w2 = None if pre_weight is None else pre_weight.contiguous()
-    hidden, normed = _BlockNorms.apply(_pitched(x, h), _pitched(branch, h), w1, w2, gate, kind, float(scale),
-                                       float(weight_offset), float(eps), float(eps if pre_eps is None else pre_eps))
-    return hidden.view(x.shape), None if normed is None else normed.view(x.shape)
+    args = (x, branch, w1, w2, gate, kind, float(scale), float(weight_offset), float(eps),
+            float(eps if pre_eps is None else pre_eps))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, branch, w1, w2, gate)):
+        hidden, normed = _BlockNorms.apply(*args)
+    else:
+        hidden = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        normed = None if w2 is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        _launch_block_norms(*args, hidden, normed, None)
+    if len(shape) != 2:
+        hidden, normed = hidden.view(shape), None if normed is None else normed.view(shape)
+    return hidden, normed
 
 
 # --------------------------------------------------------------------------- rotary position embedding
@@ -516,7 +548,7 @@ class _RopePositions(torch.autograd.Function):
         return _launch_rope_positions(q, k, pos, inv_freq, interleaved, amplitude, False)
 
     @staticmethod
-    @once_differentiable
+    @_first_derivative
     def backward(ctx, gq: Tensor | None, gk: Tensor | None):
         gq = gq if ctx.needs_input_grad[0] else None
         gk = gk if ctx.needs_input_grad[1] else None
@@ -552,8 +584,8 @@ def rope_at_positions(q: Tensor, k: Tensor | None, position_ids: Tensor, inv_fre
     so far positions keep their fraction of a turn.  `inv_freq` (fp32 or fp64) as `rope_frequencies` or a model's
     rotary module gives it.  No cos / sin tables are read or kept for the backward.  Any strides; q and k as blocks of
     a stacked projection are taken where they lie."""
-    C.require_device(q, k, position_ids, inv_freq)
     if not rope_at_positions_supported(q, k, position_ids, inv_freq):
+        C.require_device(q, k, position_ids, inv_freq)
         raise ValueError(
             "rope_at_positions: q [B, heads, T, D] and k [B, heads, T, D] or None in one dtype (bf16 or fp32), position_ids "
             "[B, T], [1, T] or [T] int64 or int32, inv_freq [r / 2] fp32 or fp64 without gradient, r <= min(D, 8192); got q "

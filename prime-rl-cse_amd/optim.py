@@ -11,6 +11,7 @@ from __future__ import annotations
 import math
 from typing import Any, Callable
 
+import numpy as np
 import torch
 from torch import nn
 from torch.optim.lr_scheduler import LambdaLR, LRScheduler
@@ -93,14 +94,15 @@ def setup_optimizer(config: Any, model: nn.Module, fused: bool | None = None, fl
 # --------------------------------------------------------------------------- gradient norm and clipping
 
 
-def _local(g: torch.Tensor) -> torch.Tensor:
-    return g.to_local() if hasattr(g, "to_local") else g
+_PIECE = np.dtype([("x", np.int64), ("n", np.int64), ("dtype", np.int32), ("reserved", np.int32)])  # prl_grad_piece
 
 
 def _sharding(grads: list[torch.Tensor]) -> list[Any] | None:
     """Process groups over which the squares of these gradients' local parts have to be added up: those of the mesh
     dimensions the gradients are sharded over ([] for plain tensors and for meshes of one rank).  None if they are
     not all plain, or all DTensors of one mesh with one placement, sharded or replicated, per mesh dimension."""
+    if all(type(g) is torch.Tensor for g in grads):
+        return []
     spread = [g for g in grads if hasattr(g, "to_local")]
     if not spread:
         return []
@@ -110,6 +112,10 @@ def _sharding(grads: list[torch.Tensor]) -> list[Any] | None:
                 or any(p.is_partial() for p in g.placements):
             return None
     return [mesh.get_group(i) for i, shard in enumerate(kinds) if shard and mesh.size(i) > 1]
+
+
+def _local_parts(grads: list[torch.Tensor]) -> list[torch.Tensor]:
+    return [g if type(g) is torch.Tensor or not hasattr(g, "to_local") else g.to_local() for g in grads]
 
 
 def _is_one_run(g: torch.Tensor) -> bool:
@@ -131,39 +137,39 @@ def clip_grad_norm_supported(grads: list[torch.Tensor]) -> bool:
         return True
     if _sharding(grads) is None:
         return False
-    parts = [_local(g) for g in grads]
+    parts = _local_parts(grads)
     dev = parts[0].device
     return dev.type == "cuda" and all(g.layout == torch.strided and g.device == dev and _is_one_run(g)
                                       and g.dtype in (torch.float32, torch.bfloat16) for g in parts)
 
 
-def _pieces(grads: list[torch.Tensor], in_place: bool) -> tuple[Any, int]:
-    """The gradients as runs of memory: a `GradPiece` array and its length.  Runs that touch end to end become one."""
-    from . import _capi as C
+_TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1}  # PRL_F32, PRL_BF16
 
-    runs: list[list[int]] = []
-    end, last = -1, None
-    for g in grads:
-        n = g.numel()
-        if n == 0:
-            continue
-        if g.layout != torch.strided or g.dtype not in (torch.float32, torch.bfloat16) or not _is_one_run(g):
+
+def _pieces(grads: list[torch.Tensor], in_place: bool) -> np.ndarray:
+    """The gradients as runs of memory: an array of `prl_grad_piece`.  Runs that touch end to end become one."""
+    codes = [_TYPE_CODES.get(g.dtype, -1) for g in grads]
+    for i, g in enumerate(grads):
+        if codes[i] < 0 or g.layout is not torch.strided or not (g.is_contiguous() or _is_one_run(g)):
             raise ValueError("gradients must be dense float32 or bfloat16 tensors that fill one run of memory, got "
                              f"{g.dtype} {g.layout} of shape {tuple(g.shape)}" +
-                             (f" with strides {g.stride()}" if g.layout == torch.strided else ""))
-        at, dtype = g.data_ptr(), g.dtype
-        if at == end and dtype is last:
-            runs[-1][1] += n
-        else:
-            runs.append([at, n, C.dtype_code(g)])
-            last = dtype
-        end = at + n * (4 if dtype is torch.float32 else 2)
-    if in_place and len(runs) > 1:
-        order = sorted(runs)
-        for a, b in zip(order, order[1:]):
-            if a[0] + a[1] * (4 if a[2] == C.PRL_F32 else 2) > b[0]:
+                             (f" with strides {g.stride()}" if g.layout is torch.strided else ""))
+    table = np.zeros(len(grads), dtype=_PIECE)
+    table["x"], table["n"], table["dtype"] = [g.data_ptr() for g in grads], [g.numel() for g in grads], codes
+    table = table[table["n"] > 0]
+    if len(table) > 1:
+        size = table["n"] * (4 - 2 * table["dtype"])
+        at = table["x"]
+        if in_place:
+            order = np.argsort(at)
+            if ((at + size)[order[:-1]] > at[order[1:]]).any():
                 raise ValueError("clip_grad_norm_: two gradients share memory (a parameter given twice?)")
-    return (C.GradPiece * max(len(runs), 1))(*[(x, n, d, 0) for x, n, d in runs]), len(runs)
+        first = np.flatnonzero(np.r_[True, ((at + size)[:-1] != at[1:]) | (table["dtype"][:-1] != table["dtype"][1:])])
+        if len(first) < len(table):
+            n = np.add.reduceat(table["n"], first)
+            table = table[first]
+            table["n"] = n
+    return table
 
 
 def _norm_kind(norm_type: float) -> int:
@@ -176,7 +182,7 @@ def _norm_kind(norm_type: float) -> int:
     raise ValueError(f"norm_type must be 2 or inf, got {norm_type}")
 
 
-def _norm_and_factor(table: Any, n: int, dev: torch.device, kind: int, max_norm: float,
+def _norm_and_factor(table: np.ndarray, dev: torch.device, kind: int, max_norm: float,
                      groups: list[Any]) -> torch.Tensor:
     """fp32 [2] on the device: the norm over `groups` and the clipping factor."""
     from . import _capi as C
@@ -184,11 +190,12 @@ def _norm_and_factor(table: Any, n: int, dev: torch.device, kind: int, max_norm:
 
     lib = C.load()
     out = torch.empty(2, dtype=torch.float32, device=dev)
-    size = lib.prl_grad_norm_workspace_bytes(table, n)
+    at, n = table.ctypes.data, len(table)
+    size = lib.prl_grad_norm_workspace_bytes(at, n)
     ws = torch.empty(size // 8 + 1, dtype=torch.float64, device=dev)  # the last one: the total
     total = ws.data_ptr() + size
     st = C.stream_ptr(dev)
-    C.check(lib.prl_grad_norm(table, n, kind, max_norm, total, out.data_ptr(), out.data_ptr() + 4, ws.data_ptr(), size,
+    C.check(lib.prl_grad_norm(at, n, kind, max_norm, total, out.data_ptr(), out.data_ptr() + 4, ws.data_ptr(), size,
                               st), "prl_grad_norm")
     if groups:
         whole = ws[-1:]
@@ -214,11 +221,11 @@ def grad_norm(grads: Any, norm_type: float = 2.0) -> torch.Tensor:
     groups = _sharding(grads)
     if groups is None:
         raise ValueError("grad_norm: plain tensors, or DTensors of one mesh placed alike (sharded or replicated)")
-    parts = [_local(g) for g in grads]
+    parts = _local_parts(grads)
     dev = C.require_device(*parts)
-    table, n = _pieces(parts, in_place=False)
+    table = _pieces(parts, in_place=False)
     with C.on_device(dev), C.timed("prl_grad_norm", dev):
-        return _norm_and_factor(table, n, dev, kind, 0.0, groups)[0]
+        return _norm_and_factor(table, dev, kind, 0.0, groups)[0]
 
 
 @torch.no_grad()
@@ -240,14 +247,14 @@ def clip_grad_norm_(parameters: Any, max_norm: float, norm_type: float = 2.0,
     groups = _sharding(grads)
     if groups is None:
         raise ValueError("clip_grad_norm_: plain gradients, or DTensors of one mesh placed alike (sharded or replicated)")
-    parts = [_local(g) for g in grads]
+    parts = _local_parts(grads)
     dev = C.require_device(*parts)
-    table, n = _pieces(parts, in_place=True)
+    table = _pieces(parts, in_place=True)
     with C.on_device(dev), C.timed("prl_clip_grad_norm", dev):
-        out = _norm_and_factor(table, n, dev, kind, float(max_norm), groups)
+        out = _norm_and_factor(table, dev, kind, float(max_norm), groups)
         if error_if_nonfinite and not math.isfinite(float(out[0])):
             raise RuntimeError(f"The total norm of order {norm_type} of the gradients is not finite, so they cannot be clipped")
-        C.check(C.load().prl_grad_scale(table, n, out.data_ptr() + 4, C.stream_ptr(dev)), "prl_grad_scale")
+        C.check(C.load().prl_grad_scale(table.ctypes.data, len(table), out.data_ptr() + 4, C.stream_ptr(dev)), "prl_grad_scale")
     return out[0]
 
 

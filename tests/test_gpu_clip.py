@@ -177,7 +177,8 @@ def test_captured_and_replayed():
 
 def test_a_total_that_ranks_have_added_up():
     g = params([((5000,), F)])[0].grad
-    table, n = optim._pieces([g], True)
+    pieces = optim._pieces([g], True)
+    table, n = pieces.ctypes.data, len(pieces)
     lib, st = C.load(), C.stream_ptr(g.device)
     ws = torch.empty(lib.prl_grad_norm_workspace_bytes(table, n) // 8, dtype=torch.float64, device=DEV)
     total, out = torch.empty(1, dtype=torch.float64, device=DEV), torch.empty(2, device=DEV)

@@ -89,9 +89,10 @@ def test_grad_entries_refuse():
 
 def test_gradients_as_runs_of_memory():
     a = torch.randn(6, 4)
-    table, n = optim._pieces([a[:2], a[2:], a.new_zeros(0), torch.randn(3).bfloat16()], True)
-    assert n == 2 and [(p.n, p.dtype) for p in table] == [(24, C.PRL_F32), (3, C.PRL_BF16)]
-    assert optim._pieces([a[3:], a[:3]], True)[1] == 2  # touching, but not in order
+    table = optim._pieces([a[:2], a[2:], a.new_zeros(0), torch.randn(3).bfloat16()], True)
+    assert [(int(p["n"]), int(p["dtype"])) for p in table] == [(24, C.PRL_F32), (3, C.PRL_BF16)]
+    assert table.dtype.itemsize == ctypes.sizeof(C.GradPiece) and len(optim._pieces([a.new_zeros(0)], True)) == 0
+    assert len(optim._pieces([a[3:], a[:3]], True)) == 2  # touching, but not in order
     assert optim._is_one_run(a.t()) and optim._is_one_run(torch.randn(3, 4, 5).permute(2, 0, 1))
     assert not optim._is_one_run(a[:, :3]) and not optim._is_one_run(a.expand(2, 6, 4))
     for bad in ([a, a], [a, a[1:2]], [a[:, 1]], [a.half()], [a.to_sparse()]):
