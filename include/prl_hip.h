@@ -552,6 +552,7 @@ int prl_adamw_flat(float* param, float* grad, float* exp_avg, float* exp_avg_sq,
  *   workspace prl_grad_norm_workspace_bytes(pieces, n_pieces), 8-byte aligned
  * prl_grad_norm_finish joins n_parts partial totals (e.g. the one all ranks have reduced) and gives total, norm and
  * coef.  prl_grad_scale multiplies every piece by coef[0] in place; where that is exactly 1 nothing is touched.
+ * prl_grad_clip is prl_grad_norm and prl_grad_scale in one call (and one launch fewer), for gradients of one process.
  * Squares are added in fp64 in an order fixed by the sizes.  A NaN anywhere gives NaN, an infinity an infinite norm.
  */
 #define PRL_NORM_L2 0
@@ -570,6 +571,8 @@ int prl_grad_norm(const prl_grad_piece* pieces, int64_t n_pieces, int kind, floa
 int prl_grad_norm_finish(const double* parts, int64_t n_parts, int kind, float max_norm, double* total, float* norm,
                          float* coef, void* stream);
 int prl_grad_scale(const prl_grad_piece* pieces, int64_t n_pieces, const float* coef, void* stream);
+int prl_grad_clip(const prl_grad_piece* pieces, int64_t n_pieces, int kind, float max_norm, float* norm, void* workspace,
+                  size_t workspace_bytes, void* stream);
 
 /*
  * Query / key RMSNorm over every head followed by the rotary embedding, reading the query and key blocks of a

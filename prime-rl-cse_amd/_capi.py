@@ -196,6 +196,7 @@ SIGNATURES = {
     "prl_grad_norm_finish": (
         c_int, [c_void_p, c_int64, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p],
     ),
+    "prl_grad_clip": (c_int, [c_void_p, c_int64, c_int, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
     "prl_grad_scale": (c_int, [c_void_p, c_int64, c_void_p, c_void_p]),
     "prl_rmsnorm_supported": (c_int, [c_int, c_int64]),
     "prl_rmsnorm_bwd_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64]),
@@ -323,6 +324,19 @@ class _OnDevice:
 
 def on_device(device: torch.device) -> _OnDevice:
     return _OnDevice(device)
+
+
+def run(fn, name: str, device: torch.device, *args) -> None:
+    """`fn(*args)` (an entry point of the library) with `device` current, timed under `name` if a timer is installed,
+    its code checked: `with on_device, timed: check(...)` without the two contexts where neither has anything to do."""
+    index = device.index
+    if _timer is None and (index is None or torch._C._cuda_getDevice() == index):
+        code = fn(*args)
+    else:
+        with on_device(device), timed(name, device):
+            code = fn(*args)
+    if code != 0:
+        check(code, name)
 
 
 def stream_ptr(device: torch.device) -> c_void_p:

@@ -240,13 +240,11 @@ def _launch_block_norms(x: Tensor, branch: Tensor, w_post: Tensor | None, w_pre:
     dev = x.device
     rows, h = x.shape
     r1 = None if rstd is None else rstd.data_ptr()
-    with C.on_device(dev), C.timed("prl_block_norms_fwd", dev):
-        C.check(C.load().prl_block_norms_fwd(
-            x.data_ptr(), x.stride(0), branch.data_ptr(), branch.stride(0),
-            None if w_post is None else w_post.data_ptr(), None if w_pre is None else w_pre.data_ptr(), kind,
-            None if gate is None else gate.data_ptr(), 0 if gate is None else gate.stride(0), scale, offset, eps_post,
-            eps_pre, hidden.data_ptr(), h, None if normed is None else normed.data_ptr(), h, r1,
-            None if r1 is None else r1 + 4 * rows, C.dtype_code(x), rows, h, C.stream_ptr(dev)), "prl_block_norms_fwd")
+    C.run(C.load().prl_block_norms_fwd, "prl_block_norms_fwd", dev, x.data_ptr(), x.stride(0), branch.data_ptr(),
+          branch.stride(0), None if w_post is None else w_post.data_ptr(), None if w_pre is None else w_pre.data_ptr(),
+          kind, None if gate is None else gate.data_ptr(), 0 if gate is None else gate.stride(0), scale, offset, eps_post,
+          eps_pre, hidden.data_ptr(), h, None if normed is None else normed.data_ptr(), h, r1,
+          None if r1 is None else r1 + 4 * rows, C.dtype_code(x), rows, h, C.stream_ptr(dev))
 
 
 class _BlockNorms(torch.autograd.Function):
@@ -255,11 +253,10 @@ class _BlockNorms(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, branch: Tensor, w_post: Tensor | None, w_pre: Tensor | None, gate: Tensor | None,
                 kind: int, scale: float, offset: float, eps_post: float, eps_pre: float):
-        dev = x.device
-        rows, h = x.shape
-        hidden = torch.empty((rows, h), dtype=x.dtype, device=dev)
-        normed = None if w_pre is None else torch.empty((rows, h), dtype=x.dtype, device=dev)
-        rstd = torch.empty(2 * rows, dtype=torch.float32, device=dev)  # of the branch, then of the sum
+        # (empty_like: rows of another pitch are given h, the cheaper call otherwise)
+        hidden = torch.empty_like(x)
+        normed = None if w_pre is None else torch.empty_like(x)
+        rstd = torch.empty(2 * x.shape[0], dtype=torch.float32, device=x.device)  # of the branch, then of the sum
         _launch_block_norms(x, branch, w_post, w_pre, gate, kind, scale, offset, eps_post, eps_pre, hidden, normed, rstd)
         ctx.save_for_backward(x, branch, w_post, w_pre, gate, rstd)
         ctx.args = (kind, scale, offset)
@@ -273,7 +270,7 @@ class _BlockNorms(torch.autograd.Function):
             return (None,) * 10
         x, branch, w_post, w_pre, gate, rstd = ctx.saved_tensors
         kind, scale, offset = ctx.args
-        dev, dtype = x.device, x.dtype
+        dev = x.device
         lib = C.load()
         rows, h = x.shape
         if gy is None:  # the normalised output went nowhere
@@ -281,24 +278,24 @@ class _BlockNorms(torch.autograd.Function):
         gh = None if gh is None else _pitched(gh, h)
         gy = None if gy is None else _pitched(gy, h)
         need = ctx.needs_input_grad
-        gx, gb = torch.empty((rows, h), dtype=dtype, device=dev), torch.empty((rows, h), dtype=dtype, device=dev)
+        gx, gb = torch.empty_like(x), torch.empty_like(x)
         g1 = torch.empty_like(w_post) if w_post is not None and need[2] else None
         g2 = torch.empty_like(w_pre) if w_pre is not None and need[3] else None
-        gg = torch.empty(gate.shape, dtype=dtype, device=dev) if gate is not None and need[4] else None
+        gg = torch.empty(gate.shape, dtype=x.dtype, device=dev) if gate is not None and need[4] else None
         code = C.dtype_code(x)
         ws, ws_bytes = None, 0
         if g1 is not None or g2 is not None or (gg is not None and kind in (C.GATE_CHANNEL, C.GATE_ONE)):
             ws_bytes = lib.prl_block_norms_bwd_workspace_bytes(code, rows, h)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        at = lambda t: None if t is None else t.data_ptr()
-        pitch = lambda t: 0 if t is None else t.stride(0)
         r1 = rstd.data_ptr()
-        with C.on_device(dev), C.timed("prl_block_norms_bwd", dev):
-            C.check(lib.prl_block_norms_bwd(
-                x.data_ptr(), x.stride(0), branch.data_ptr(), branch.stride(0), at(w_post), at(w_pre), kind, at(gate),
-                pitch(gate), scale, offset, r1, r1 + 4 * rows, at(gh), pitch(gh), at(gy), pitch(gy), gx.data_ptr(), h,
-                gb.data_ptr(), h, at(g1), at(g2), at(gg), pitch(gg), code, rows, h, at(ws), ws_bytes,
-                C.stream_ptr(dev)), "prl_block_norms_bwd")
+        C.run(lib.prl_block_norms_bwd, "prl_block_norms_bwd", dev, x.data_ptr(), x.stride(0), branch.data_ptr(),
+              branch.stride(0), None if w_post is None else w_post.data_ptr(), None if w_pre is None else w_pre.data_ptr(),
+              kind, None if gate is None else gate.data_ptr(), 0 if gate is None else gate.stride(0), scale, offset, r1,
+              r1 + 4 * rows, None if gh is None else gh.data_ptr(), 0 if gh is None else gh.stride(0),
+              None if gy is None else gy.data_ptr(), 0 if gy is None else gy.stride(0), gx.data_ptr(), h, gb.data_ptr(), h,
+              None if g1 is None else g1.data_ptr(), None if g2 is None else g2.data_ptr(),
+              None if gg is None else gg.data_ptr(), 0 if gg is None else gg.stride(0), code, rows, h,
+              None if ws is None else ws.data_ptr(), ws_bytes, C.stream_ptr(dev))
         return gx, gb, g1, g2, gg, None, None, None, None, None
 
 
@@ -345,8 +342,7 @@ def block_norms(x: Tensor, branch: Tensor, post_weight: Tensor | None = None, pr
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, branch, w1, w2, gate)):
         hidden, normed = _BlockNorms.apply(*args)
     else:
-        hidden = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        normed = None if w2 is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        hidden, normed = torch.empty_like(x), None if w2 is None else torch.empty_like(x)
         _launch_block_norms(*args, hidden, normed, None)
     if len(shape) != 2:
         hidden, normed = hidden.view(shape), None if normed is None else normed.view(shape)
@@ -531,11 +527,9 @@ def _launch_rope_positions(q: Tensor | None, k: Tensor | None, pos: Tensor, inv_
         args += [x.data_ptr(), out.data_ptr(), _strides6(x, out), x.shape[1]]
     if 0 in (b, t) or args[3] + args[7] == 0:
         return outs[0], outs[1]
-    with C.on_device(dev), C.timed("prl_rope_positions", dev):
-        C.check(C.load().prl_rope_positions(
-            *args, pos.data_ptr(), pos.dtype == torch.int64, pos.stride(0) if pos.shape[0] > 1 else 0, pos.stride(1),
-            inv_freq.data_ptr(), inv_freq.dtype == torch.float64, 2 * inv_freq.numel(), interleaved, amplitude,
-            C.dtype_code(one), b, t, d, inverse, C.stream_ptr(dev)), "prl_rope_positions")
+    C.run(C.load().prl_rope_positions, "prl_rope_positions", dev, *args, pos.data_ptr(), pos.dtype is torch.int64,
+          pos.stride(0) if pos.shape[0] > 1 else 0, pos.stride(1), inv_freq.data_ptr(), inv_freq.dtype is torch.float64,
+          2 * inv_freq.numel(), interleaved, amplitude, C.dtype_code(one), b, t, d, inverse, C.stream_ptr(dev))
     return outs[0], outs[1]
 
 

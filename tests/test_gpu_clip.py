@@ -188,3 +188,11 @@ def test_a_total_that_ranks_have_added_up():
     want = g.double().norm() * math.sqrt(2.0)
     assert abs(float(out[0]) - float(want)) <= 2.0**-23 * float(want)
     assert abs(float(out[1]) - 1.0 / (float(want) + 1e-6)) <= 2.0**-22 / float(want)
+
+
+@pytest.mark.parametrize("which", ["small", "many", "larger"])
+def test_one_call_and_its_two_halves_agree(which):
+    a, b = params(SHAPES[which]), params(SHAPES[which])
+    n1 = optim.clip_grad_norm_(a, 0.5)
+    n2 = optim.clip_grad_norm_(b, 0.5, error_if_nonfinite=True)
+    assert torch.equal(n1, n2) and all(torch.equal(p.grad, q.grad) for p, q in zip(a, b))

@@ -76,11 +76,13 @@ def test_grad_entries_refuse():
         t = (C.GradPiece * 1)(bad)
         assert lib.prl_grad_norm(t, 1, 0, 1.0, ONE, ONE, ONE, ONE, 1 << 20, None) == -1
         assert lib.prl_grad_scale(t, 1, ONE, None) == -1
+        assert lib.prl_grad_clip(t, 1, 0, 1.0, ONE, ONE, 1 << 20, None) == -1
         assert lib.prl_grad_norm_workspace_bytes(t, 1) == 0
     assert lib.prl_grad_norm(ok, 2, 2, 1.0, ONE, ONE, ONE, ONE, 64, None) == -1
     assert lib.prl_grad_norm(ok, 2, 0, 1.0, None, None, None, ONE, 64, None) == -1
     assert lib.prl_grad_norm(ok, 2, 0, 1.0, ONE, ONE, ONE, ONE, 4, None) == -1
     assert lib.prl_grad_norm(ok, -1, 0, 1.0, ONE, ONE, ONE, ONE, 64, None) == -1
+    assert lib.prl_grad_clip(ok, 2, 0, 1.0, None, ONE, 64, None) == -1 and lib.prl_grad_clip(ok, 2, 0, 1.0, ONE, ONE, 4, None) == -1
     assert lib.prl_grad_scale(ok, 2, None, None) == -1 and lib.prl_grad_scale(ok, 0, ONE, None) == 0
     assert lib.prl_grad_norm_finish(None, 1, 0, 1.0, ONE, ONE, ONE, None) == -1
     big = (C.GradPiece * 300)(*[(16, 1 << 20, i % 2, 0) for i in range(300)])
