@@ -11,25 +11,15 @@
 // It is formed in fp64 in turns, p f / (2 pi), and only its fraction of a turn goes to fp32, where sincospi is good to
 // fp32 rounding.
 //
-// Bound by HBM: every element read and written once.  A workgroup takes a few tokens, forms their cos / sin once in
-// LDS (r / 2 pairs per token) and uses them for all heads of query and key.
+// Bound by HBM: every element read and written once.  A workgroup takes a few tokens and forms their cos / sin once in
+// LDS (r / 2 pairs per token).  A thread then owns one place in the head, two 16-byte vectors of it, keeps its cos / sin
+// in registers and walks over the heads of query and key, two at a time: no index arithmetic between heads.
 #include "logprob_dev.h"
 
 namespace prl {
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeMaxPairs = 4096;  // r / 2 at most: 32 KB of LDS per token
-
-// n / d for n < 2^31 without a division: (mulhi(n, mul) + n) >> shift, exact for every such n.
-struct FastDiv {
-  uint32_t d, mul, shift;
-};
-static FastDiv fast_div(uint32_t d) {
-  uint32_t s = 0;
-  while ((1ull << s) < d) ++s;
-  return {d, (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1), s};
-}
-__device__ __forceinline__ uint32_t quotient(uint32_t n, const FastDiv& f) { return (__umulhi(n, f.mul) + n) >> f.shift; }
 
 // The fraction of a turn that p f radians are, in [-1/2, 1/2].  p f / (2 pi) is carried as a sum of two doubles (1 / (2 pi)
 // to twice their length, the products' remainders by fma), so that what is left after the whole turns is good to fp32
@@ -47,64 +37,77 @@ struct RopeSide {
   int64_t xb, xh, xt, ob, oh, ot;  // strides in bytes
 };
 
-// 16 bytes at an address that is only aligned to an element
-typedef unsigned int u32x4_e2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef unsigned int u32x4_e4 __attribute__((ext_vector_type(4), aligned(4)));
+// VEC: a thread's two pieces of a head are 16-byte vectors (rows aligned, the pairs of the half layout in whole vectors);
+// otherwise single elements, side by side over the lanes (r = 34 of 128 in the half layout:
+// 53.5 us; 16-byte accesses at places aligned to an element only took 107).
+template <int DT, bool VEC>
+struct RopeUnit {
+  static constexpr int kEs = DT == PRL_F32 ? 4 : 2;
+  static constexpr int kN = VEC ? 16 / kEs : 1;  // elements of a piece
+  u32x4 z;
+  __device__ __forceinline__ void load(const char* p) {
+    if constexpr (VEC) z = *reinterpret_cast<const u32x4*>(p);
+    else if constexpr (DT == PRL_F32) z.x = *reinterpret_cast<const uint32_t*>(p);
+    else z.x = *reinterpret_cast<const uint16_t*>(p);
+  }
+  __device__ __forceinline__ void get(float* y) const {
+    if constexpr (VEC) decode16_raw<DT>(z, y);
+    else y[0] = DT == PRL_F32 ? __uint_as_float(z.x) : bf16_lo(z.x);
+  }
+  __device__ __forceinline__ void store(char* p) const {
+    if constexpr (VEC) *reinterpret_cast<u32x4*>(p) = z;
+    else if constexpr (DT == PRL_F32) *reinterpret_cast<uint32_t*>(p) = z.x;
+    else *reinterpret_cast<uint16_t*>(p) = (uint16_t)z.x;
+  }
+  __device__ __forceinline__ void put(const float* y) {
+    if constexpr (!VEC) z.x = DT == PRL_F32 ? __float_as_uint(y[0]) : one_bf16(y[0]);
+    else if constexpr (DT == PRL_F32)
+      z.x = __float_as_uint(y[0]), z.y = __float_as_uint(y[1]), z.z = __float_as_uint(y[2]), z.w = __float_as_uint(y[3]);
+    else
+      z.x = pack_bf16(y[0], y[1]), z.y = pack_bf16(y[2], y[3]), z.z = pack_bf16(y[4], y[5]), z.w = pack_bf16(y[6], y[7]);
+  }
+};
 
-// `n` of the VE elements from p on (n < VE: the rest is 0 and not read)
-template <int DT, bool AL>
-__device__ __forceinline__ void rope_load(const char* p, int n, float* y) {
-  constexpr int VE = DT == PRL_F32 ? 4 : 8;
-  if (n >= VE) {
-    u32x4 v;
-    if constexpr (AL) v = *reinterpret_cast<const u32x4*>(p);
-    else if constexpr (DT == PRL_F32) v = *reinterpret_cast<const u32x4_e4*>(p);
-    else v = *reinterpret_cast<const u32x4_e2*>(p);
-    decode16_raw<DT>(v, y);
-    return;
-  }
+struct RopeShape {
+  int r, D;         // rotated dimensions, head size
+  int units;        // places in a head: pairs of pieces
+  int per_row;      // threads side by side on a row: min(units, threads)
+  int slots, toks;  // heads and tokens a workgroup has in flight
+};
+
+// Turns the two pieces of one head in place; `turn` bit e: pair e belongs to the rotated part.
+template <int DT, bool IL, bool VEC>
+__device__ __forceinline__ void rope_turn(RopeUnit<DT, VEC>& p1, RopeUnit<DT, VEC>& p2, const float* c, const float* s,
+                                          uint32_t turn) {
+  constexpr int N = RopeUnit<DT, VEC>::kN;
+  if (!turn) return;
+  float x[2 * N], y[2 * N];
+  p1.get(x), p2.get(x + N);
 #pragma unroll
-  for (int i = 0; i < VE; ++i) {
-    y[i] = 0.0f;
-    if (i < n) y[i] = DT == PRL_F32 ? reinterpret_cast<const float*>(p)[i] : bf16_one(reinterpret_cast<const uint16_t*>(p)[i]);
+  for (int e = 0; e < N; ++e) {
+    const int i = IL ? 2 * e : e, j = IL ? 2 * e + 1 : e + N;
+    const bool on = !IL || (turn >> e & 1);
+    y[i] = on ? fmaf(x[i], c[e], -(x[j] * s[e])) : x[i];
+    y[j] = on ? fmaf(x[j], c[e], x[i] * s[e]) : x[j];
   }
-}
-template <int DT, bool AL>
-__device__ __forceinline__ void rope_store(char* p, int n, const float* y) {
-  constexpr int VE = DT == PRL_F32 ? 4 : 8;
-  if (n >= VE) {
-    u32x4 v;
-    if constexpr (DT == PRL_F32) {
-      v.x = __float_as_uint(y[0]), v.y = __float_as_uint(y[1]), v.z = __float_as_uint(y[2]), v.w = __float_as_uint(y[3]);
-    } else {
-      v.x = pack_bf16(y[0], y[1]), v.y = pack_bf16(y[2], y[3]), v.z = pack_bf16(y[4], y[5]), v.w = pack_bf16(y[6], y[7]);
-    }
-    if constexpr (AL) *reinterpret_cast<u32x4*>(p) = v;
-    else if constexpr (DT == PRL_F32) *reinterpret_cast<u32x4_e4*>(p) = v;
-    else *reinterpret_cast<u32x4_e2*>(p) = v;
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < VE; ++i)
-    if (i < n) store_elem<DT>(p, i, y[i]);
+  p1.put(y), p2.put(y + N);
 }
 
-// One row of a head is `rot` units of rotation (VE pairs of the half layout, VE / 2 of the interleaved one) and then
-// the units of VE elements that pass through; a unit at the end of either part may be shorter.
-template <int DT, bool IL, bool AL>
-__global__ __launch_bounds__(kRopeThreads) void k_rope_positions(
-    RopeSide q, RopeSide k, int q_heads, FastDiv heads, FastDiv units, FastDiv per_batch, int rot,
-    const char* __restrict__ pos, int pos64, int64_t pos_b, int64_t pos_t, const char* __restrict__ inv_freq, int freq64,
-    int r, int D, float amplitude, int inverse, int n_tokens, int tok_per_wg) {
-  constexpr int ES = DT == PRL_F32 ? 4 : 2;
-  constexpr int VE = 16 / ES;
+template <int DT, bool IL, bool VEC>
+__global__ __launch_bounds__(kRopeThreads) void k_rope_positions(RopeSide q, RopeSide k, int q_heads, int heads,
+                                                                 RopeShape sh, const char* __restrict__ pos, int pos64,
+                                                                 int64_t pos_b, int64_t pos_t,
+                                                                 const char* __restrict__ inv_freq, int freq64,
+                                                                 float amplitude, int inverse, int n_tokens, int T) {
+  using P = RopeUnit<DT, VEC>;
+  constexpr int N = P::kN, ES = P::kEs;
   extern __shared__ float2 cs[];  // [token of the workgroup][pair]
-  const int half = r >> 1;
-  const int tok0 = blockIdx.x * tok_per_wg;
-  const int ntok = min(tok_per_wg, n_tokens - tok0);
+  const int half = sh.r >> 1;
+  const int tok0 = blockIdx.x * sh.toks;
+  const int ntok = min(sh.toks, n_tokens - tok0);
   for (int i = threadIdx.x; i < ntok * half; i += kRopeThreads) {
     const int tok = i / half, j = i - tok * half;
-    const uint32_t n = tok0 + tok, b = quotient(n, per_batch), t = n - b * per_batch.d;
+    const int n = tok0 + tok, b = n / T, t = n - b * T;
     const char* pp = pos + b * pos_b + t * pos_t;
     const double p = pos64 ? (double)*reinterpret_cast<const int64_t*>(pp) : (double)*reinterpret_cast<const int32_t*>(pp);
     const double f = freq64 ? reinterpret_cast<const double*>(inv_freq)[j] : (double)reinterpret_cast<const float*>(inv_freq)[j];
@@ -113,46 +116,77 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope_positions(
     cs[i] = make_float2(c * amplitude, (inverse ? -s : s) * amplitude);
   }
   __syncthreads();
-  const uint32_t per_tok = heads.d * units.d;
-  for (uint32_t i = threadIdx.x; i < ntok * per_tok; i += kRopeThreads) {
-    const uint32_t row = quotient(i, units), u = i - row * units.d;
-    const uint32_t tok = quotient(row, heads), h = row - tok * heads.d;
-    const uint32_t n = tok0 + tok, b = quotient(n, per_batch), t = n - b * per_batch.d;
-    const RopeSide& a = (int)h < q_heads ? q : k;
-    const int64_t hh = (int)h < q_heads ? h : h - q_heads;
-    const char* xp = a.x + b * a.xb + hh * a.xh + t * a.xt;
-    char* op = a.out + b * a.ob + hh * a.oh + t * a.ot;
-    float x1[VE], x2[VE], o1[VE], o2[VE];
-    if ((int)u >= rot) {  // the part of the head that passes through
-      const int at = r + ((int)u - rot) * VE, left = D - at;
-      rope_load<DT, AL>(xp + (int64_t)at * ES, left, x1);
-      rope_store<DT, AL>(op + (int64_t)at * ES, left, x1);
-    } else if (IL) {
-      const int at = (int)u * VE, left = r - at;
-      const float2* w = cs + tok * half + at / 2;
-      rope_load<DT, AL>(xp + at * ES, left, x1);
-#pragma unroll
-      for (int e = 0; e < VE; e += 2) {
-        const float2 z = e < left ? w[e / 2] : make_float2(0.0f, 0.0f);
-        o1[e] = fmaf(x1[e], z.x, -(x1[e + 1] * z.y));
-        o1[e + 1] = fmaf(x1[e + 1], z.x, x1[e] * z.y);
-      }
-      rope_store<DT, AL>(op + at * ES, left, o1);
+  const int g = threadIdx.x / sh.per_row, u0 = threadIdx.x - g * sh.per_row;
+  const int tok = g / sh.slots, h0 = g - tok * sh.slots;
+  if (tok >= ntok) return;
+  const int n = tok0 + tok;
+  const int64_t b = n / T, t = n - b * T;
+  for (int u = u0; u < sh.units; u += sh.per_row) {
+    // the two pieces' first elements, and which of their pairs turn
+    int e1, e2, pair;
+    uint32_t turn;
+    if (IL) {
+      e1 = 2 * N * u, e2 = e1 + N, pair = N * u;
+      const int on = half - pair;
+      turn = on >= N ? (1u << N) - 1 : on > 0 ? (1u << on) - 1 : 0;
     } else {
-      const int at = (int)u * VE, left = half - at;
-      const float2* w = cs + tok * half + at;
-      rope_load<DT, AL>(xp + at * ES, left, x1);
-      rope_load<DT, AL>(xp + (at + half) * ES, left, x2);
+      const int rot = half / N;
+      pair = N * u;
+      turn = u < rot;
+      e1 = turn ? pair : sh.r + 2 * N * (u - rot), e2 = turn ? half + pair : e1 + N;
+    }
+    const bool two = e2 < sh.D;
+    float c[N], s[N];
+    if (turn) {
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const float2 z = e < left ? w[e] : make_float2(0.0f, 0.0f);
-        o1[e] = fmaf(x1[e], z.x, -(x2[e] * z.y));
-        o2[e] = fmaf(x2[e], z.x, x1[e] * z.y);
+      for (int e = 0; e < N; ++e) {
+        const float2 z = cs[tok * half + (IL ? min(pair + e, half - 1) : pair + e)];
+        c[e] = z.x, s[e] = z.y;
       }
-      rope_store<DT, AL>(op + at * ES, left, o1);
-      rope_store<DT, AL>(op + (at + half) * ES, left, o2);
+    }
+    const char* xq = q.x + b * q.xb + t * q.xt + (int64_t)e1 * ES;
+    const char* xk = k.x + b * k.xb + t * k.xt + (int64_t)e1 * ES;
+    char* oq = q.out + b * q.ob + t * q.ot + (int64_t)e1 * ES;
+    char* ok = k.out + b * k.ob + t * k.ot + (int64_t)e1 * ES;
+    const int64_t gap = (int64_t)(two ? e2 - e1 : 0) * ES;  // (a last piece alone is loaded twice and stored once)
+    for (int h = h0; h < heads; h += 2 * sh.slots) {
+      const int g2 = h + sh.slots;
+      const bool also = g2 < heads;
+      const char *xa = h < q_heads ? xq + h * q.xh : xk + (h - q_heads) * k.xh, *xb = xa;
+      char *oa = h < q_heads ? oq + h * q.oh : ok + (h - q_heads) * k.oh, *ob = oa;
+      if (also) {
+        xb = g2 < q_heads ? xq + g2 * q.xh : xk + (g2 - q_heads) * k.xh;
+        ob = g2 < q_heads ? oq + g2 * q.oh : ok + (g2 - q_heads) * k.oh;
+      }
+      P a1, a2, b1, b2;
+      a1.load(xa), a2.load(xa + gap);
+      if (also) b1.load(xb), b2.load(xb + gap);
+      rope_turn<DT, IL, VEC>(a1, a2, c, s, turn);
+      a1.store(oa);
+      if (two) a2.store(oa + gap);
+      if (also) {
+        rope_turn<DT, IL, VEC>(b1, b2, c, s, turn);
+        b1.store(ob);
+        if (two) b2.store(ob + gap);
+      }
     }
   }
+}
+
+// Threads of a workgroup: `units` side by side on a row as far as they go, the rest over two tokens and as many heads of
+// each as fit (16384 tokens of 24 heads of 128 bf16, 201 MB: 41.1 us with two tokens, 49.0 with one, 42.3 with four;
+// 48 single tokens: 4.2 us with one, two or four).
+static RopeShape rope_shape(int64_t r, int64_t D, int64_t heads, int ve, bool il, bool vec) {
+  RopeShape s;
+  s.r = (int)r, s.D = (int)D;
+  const int64_t n = vec ? ve : 1;
+  s.units = (int)(il ? (D + 2 * n - 1) / (2 * n) : r / 2 / n + (D - r + 2 * n - 1) / (2 * n));
+  s.per_row = s.units < kRopeThreads ? s.units : kRopeThreads;
+  const int groups = kRopeThreads / s.per_row;
+  int toks = groups < 2 || r / 2 > kRopeMaxPairs / 2 ? 1 : 2;
+  s.slots = groups / toks < heads ? groups / toks : (int)heads;
+  s.toks = groups / s.slots < toks ? groups / s.slots : toks;
+  return s;
 }
 
 }  // namespace prl
@@ -181,12 +215,9 @@ extern "C" int prl_rope_positions(const void* q, void* q_out, const int64_t* q_s
   PRL_REQUIRE(positions && inv_freq, "rope_positions: positions and inv_freq must not be NULL");
   PRL_REQUIRE(q_heads == 0 || (q && q_out && q_strides), "rope_positions: q, q_out and q_strides must not be NULL");
   PRL_REQUIRE(k_heads == 0 || (k && k_out && k_strides), "rope_positions: k, k_out and k_strides must not be NULL");
-  const int64_t half = rotary_dim / 2;
-  const int64_t rot = interleaved ? (rotary_dim + ve - 1) / ve : (half + ve - 1) / ve;
-  const int64_t units = rot + (D - rotary_dim + ve - 1) / ve;
-  const int64_t heads = q_heads + k_heads;
+  const int64_t half = rotary_dim / 2, heads = q_heads + k_heads;
   PRL_REQUIRE(B < (1ll << 31) && T < (1ll << 31) && B * T < (1ll << 31) - 64, "rope_positions: B * T must be below 2^31");
-  PRL_REQUIRE(heads < (1ll << 20) && units * heads < (1ll << 26), "rope_positions: too many heads");
+  PRL_REQUIRE(heads < (1ll << 20), "rope_positions: too many heads");
   uintptr_t bits = 0, elem = 0;
   RopeSide side[2] = {};
   const void* in[2] = {q, k};
@@ -203,26 +234,24 @@ extern "C" int prl_rope_positions(const void* q, void* q_out, const int64_t* q_s
   }
   PRL_REQUIRE((elem & (es - 1)) == 0, "rope_positions: pointers must be aligned to an element");
   // every 16-byte access of a row starts a multiple of 16 bytes from the row's start
-  const bool al = ((bits | (uintptr_t)(rotary_dim * es) | (uintptr_t)(interleaved ? 0 : half * es)) & 15) == 0;
+  const bool vec = ((bits | (uintptr_t)(D * es) | (uintptr_t)(interleaved ? 0 : half * es)) & 15) == 0;
   const int64_t tokens = B * T;
-  int tok = 1;
-  const int64_t grid = (tokens + tok - 1) / tok;
-  const size_t lds = (size_t)tok * half * sizeof(float2);
-#define PRL_ROPE(DT, IL, AL)                                                                                         \
-  hipLaunchKernelGGL((k_rope_positions<DT, IL, AL>), dim3((unsigned)grid), dim3(kRopeThreads), lds, (hipStream_t)stream, \
-                     side[0], side[1], (int)q_heads, fast_div((uint32_t)heads), fast_div((uint32_t)units),           \
-                     fast_div((uint32_t)T), (int)rot, (const char*)positions, positions_64 ? 1 : 0,                  \
+  const RopeShape sh = rope_shape(rotary_dim, D, heads, ve, interleaved, vec);
+  const int64_t grid = (tokens + sh.toks - 1) / sh.toks;
+  const size_t lds = (size_t)sh.toks * half * sizeof(float2);
+#define PRL_ROPE(DT, IL, VEC)                                                                                       \
+  hipLaunchKernelGGL((k_rope_positions<DT, IL, VEC>), dim3((unsigned)grid), dim3(kRopeThreads), lds, (hipStream_t)stream, \
+                     side[0], side[1], (int)q_heads, (int)heads, sh, (const char*)positions, positions_64 ? 1 : 0,   \
                      pos_batch_stride * (positions_64 ? 8 : 4), pos_token_stride * (positions_64 ? 8 : 4),           \
-                     (const char*)inv_freq, inv_freq_64 ? 1 : 0, (int)rotary_dim, (int)D, amplitude, inverse ? 1 : 0, \
-                     (int)tokens, tok)
-#define PRL_ROPE_AL(DT, IL) \
-  if (al) PRL_ROPE(DT, IL, true); else PRL_ROPE(DT, IL, false)
+                     (const char*)inv_freq, inv_freq_64 ? 1 : 0, amplitude, inverse ? 1 : 0, (int)tokens, (int)T)
+#define PRL_ROPE_VEC(DT, IL) \
+  if (vec) PRL_ROPE(DT, IL, true); else PRL_ROPE(DT, IL, false)
   if (dtype == PRL_BF16) {
-    if (interleaved) { PRL_ROPE_AL(PRL_BF16, true); } else { PRL_ROPE_AL(PRL_BF16, false); }
+    if (interleaved) { PRL_ROPE_VEC(PRL_BF16, true); } else { PRL_ROPE_VEC(PRL_BF16, false); }
   } else {
-    if (interleaved) { PRL_ROPE_AL(PRL_F32, true); } else { PRL_ROPE_AL(PRL_F32, false); }
+    if (interleaved) { PRL_ROPE_VEC(PRL_F32, true); } else { PRL_ROPE_VEC(PRL_F32, false); }
   }
-#undef PRL_ROPE_AL
+#undef PRL_ROPE_VEC
 #undef PRL_ROPE
   PRL_CHECK_LAUNCH("rope_positions");
   return PRL_OK;
