@@ -418,6 +418,87 @@ def apply_rotary_pos_emb(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, unsquee
     return _ORIGINAL_ROPE[0](q, k, cos, sin, unsqueeze_dim)
 
 
+class _RopeSource:
+    """Where a rotary module's cos / sin came from: what `rope_at_positions` takes instead of them."""
+
+    __slots__ = ("position_ids", "inv_freq", "amplitude")
+
+    def __init__(self, position_ids: Tensor, inv_freq: Tensor, amplitude: float):
+        self.position_ids, self.inv_freq, self.amplitude = position_ids, inv_freq, amplitude
+
+
+def _tagged_rotary_forward(self: nn.Module, x: Tensor, position_ids: Tensor, *args: Any, **kwargs: Any):
+    """A rotary module's own forward, with its positions and frequencies left on the cos it returns for the attention
+    blocks' rotary function (`_family_rope`), which gets that very tensor."""
+    cos, sin = self._prl_torch_forward(x, position_ids, *args, **kwargs)
+    inv_freq = self.inv_freq  # (read after the call: frequencies that depend on the length are set in there)
+    if inv_freq.dtype != torch.float32:
+        inv_freq = inv_freq.float()  # as the module itself uses it
+    cos._prl_rope = _RopeSource(position_ids, inv_freq, float(getattr(self, "attention_scaling", 1.0)))
+    return cos, sin
+
+
+def _family_rope(original: Any, kind: str) -> Any:
+    """The rotary function of a model family whose pairs lie as `kind` says ("half" or "interleaved"): the table kernel
+    for whole heads in the half layout, the kernel that works from positions for the others where the tables come
+    from a tagged rotary module, the family's own function for everything else."""
+
+    def rotate(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, *args: Any, **kwargs: Any):
+        if not args and not kwargs or (kwargs == {"unsqueeze_dim": 1} and not args) or (args == (1,) and not kwargs):
+            source = getattr(cos, "_prl_rope", None)
+            if source is None:
+                if kind == "half" and rope_supported(q, k, cos, sin):
+                    return _Rope.apply(q, k, cos, sin)
+            elif rope_at_positions_supported(q, k, source.position_ids, source.inv_freq):
+                return rope_at_positions(q, k, source.position_ids, source.inv_freq, interleaved=kind == "interleaved",
+                                         attention_scaling=source.amplitude)
+        return original(q, k, cos, sin, *args, **kwargs)
+
+    return rotate
+
+
+def _rope_kind(home: Any, model: nn.Module) -> tuple[str, list[nn.Module]] | None:
+    """How a family's `apply_rotary_pos_emb` pairs the dimensions of a head, found by what it does to a small host
+    tensor, and the rotary modules to tag (none for whole heads in the half layout, which have their tables); None for
+    a function that does something else."""
+    import copy
+
+    original = home.apply_rotary_pos_emb
+    modules = [m for m in model.modules() if type(m).__name__.endswith("RotaryEmbedding")
+               and isinstance(getattr(m, "inv_freq", None), Tensor)]
+    config = getattr(model, "config", None)
+    heads = getattr(config, "num_attention_heads", None)
+    size = getattr(config, "head_dim", None) or (config.hidden_size // heads if heads else None)
+    if not modules or modules[0].inv_freq.is_meta or size is None:
+        try:  # no tables to be had: the pairs are told by the helper that these families have
+            turned = home.rotate_half(torch.arange(4.0)).tolist()
+        except Exception:
+            return "half", []
+        return ("half", []) if turned == [-2.0, -3.0, 0.0, 1.0] else None
+    rotary = copy.deepcopy(modules[0])
+    rotary.forward = types.MethodType(type(rotary).forward, rotary)
+    rotary = rotary.cpu().float()
+    gen = torch.Generator().manual_seed(0)
+    pos = torch.tensor([[3, 4, 5, 11, 2]])
+    r = 2 * rotary.inv_freq.numel()
+    for d in dict.fromkeys((size, r)):
+        q, k = torch.randn(1, 2, 5, d, generator=gen), torch.randn(1, 1, 5, d, generator=gen)
+        try:
+            with torch.no_grad():
+                cos, sin = rotary(q, pos)
+                got = original(q, k, cos, sin)[0]
+        except Exception:
+            continue
+        theta = (pos[..., None] * rotary.inv_freq)[:, None]
+        c, s = theta.cos() * getattr(rotary, "attention_scaling", 1.0), theta.sin() * getattr(rotary, "attention_scaling", 1.0)
+        for kind in ("half", "interleaved"):
+            u, v = (q[..., : r // 2], q[..., r // 2 : r]) if kind == "half" else (q[..., 0:r:2], q[..., 1:r:2])
+            a, b = u * c - v * s, v * c + u * s
+            want = torch.cat([a, b], -1) if kind == "half" else torch.stack([a, b], -1).flatten(-2)
+            if got.shape == q.shape and torch.allclose(got, torch.cat([want, q[..., r:]], -1), rtol=1e-4, atol=1e-5):
+                return kind, [] if kind == "half" and size == r else modules
+    return None
+
 
 def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict[str, Any] | None = None,
                      max_position_embeddings: int | None = None, seq_len: int | None = None,
@@ -927,7 +1008,174 @@ def _is_plain_decoder_layer(module: nn.Module) -> bool:
             pos = body.index(want, pos) + 1
         except ValueError:
             return False
+    # a norm behind a block would be one more step of this form (such layers: `_layer_steps`)
+    if sum(ln.startswith("hidden_states = self.") for ln in body) != 3:
+        return False
     return body.count("hidden_states = residual + hidden_states") == 2 and body.count("residual = hidden_states") == 2
+
+
+
+class _LayerSteps:
+    """A decoder layer's forward as steps, read from its source: norm before the attention (or None), after it, the
+    factor on the branch (an attribute's name or None), then the same around the MLP."""
+
+    __slots__ = ("signature", "attention", "pre1", "post1", "scale1", "pre2", "post2", "scale2")
+
+
+def _layer_steps(module: nn.Module) -> _LayerSteps | None:
+    """The steps of a decoder layer whose forward is residual, [norm], attention, [norm], scaled addition, residual,
+    [norm], MLP, [norm], scaled addition, and nothing else; None for any other.  Layers of the plain shape
+    (`_is_plain_decoder_layer`) are not taken here: their additions round as the separate modules do."""
+    import ast
+    import inspect
+    import textwrap
+
+    if not type(module).__name__.endswith("DecoderLayer") or not all(hasattr(module, a) for a in ("self_attn", "mlp")):
+        return None
+    try:
+        tree = ast.parse(textwrap.dedent(inspect.getsource(type(module).forward))).body[0]
+        steps = _LayerSteps()
+        steps.signature = inspect.signature(type(module).forward)
+    except (OSError, TypeError, SyntaxError, ValueError):
+        return None
+    body = [st for st in tree.body if not (isinstance(st, ast.Expr) and isinstance(st.value, ast.Constant))]
+    tokens: list[tuple[str, Any]] = []
+    for st in body:
+        if isinstance(st, ast.Return):
+            tokens.append(("return", ast.unparse(st.value)))
+            continue
+        if not isinstance(st, ast.Assign) or len(st.targets) != 1:
+            return None
+        target, value = ast.unparse(st.targets[0]).strip("()"), st.value
+        if isinstance(value, ast.Call) and ast.unparse(value.func).startswith("self."):
+            name = ast.unparse(value.func)[5:]
+            if name == "self_attn":
+                if target not in ("hidden_states, _", "hidden_states, self_attn_weights") or value.args:
+                    return None
+                tokens.append(("attention", [(kw.arg, ast.unparse(kw.value)) for kw in value.keywords]))
+                continue
+            if target != "hidden_states" or [ast.unparse(a) for a in value.args] != ["hidden_states"] or value.keywords:
+                return None
+            tokens.append(("mlp" if name == "mlp" else "norm", name))
+            continue
+        text = f"{target} = {ast.unparse(value)}"
+        if text == "residual = hidden_states":
+            tokens.append(("residual", None))
+        elif text == "hidden_states = residual + hidden_states":
+            tokens.append(("add", None))
+        elif text == "hidden_states = residual + hidden_states * self.residual_multiplier":
+            tokens.append(("add", "residual_multiplier"))
+        else:
+            return None
+    at = 0
+
+    def take(kind: str, optional: bool = False) -> Any:
+        nonlocal at
+        if at < len(tokens) and tokens[at][0] == kind:
+            at += 1
+            return tokens[at - 1][1] if tokens[at - 1][1] is not None else True
+        return None if optional else False
+
+    if take("residual") is False:
+        return None
+    steps.pre1 = take("norm", True)
+    steps.attention = take("attention")
+    steps.post1 = take("norm", True)
+    scale1 = take("add")
+    if steps.attention is False or scale1 is False or take("residual") is False:
+        return None
+    steps.pre2 = take("norm", True)
+    if take("mlp") is False:
+        return None
+    steps.post2 = take("norm", True)
+    scale2 = take("add")
+    if scale2 is False or take("return") != "hidden_states" or at != len(tokens):
+        return None
+    steps.scale1, steps.scale2 = (None if sc is True else sc for sc in (scale1, scale2))
+    names = {kw for kw, _ in steps.attention if kw}
+    params = steps.signature.parameters
+    if "hidden_states" not in names or any(v not in params for _, v in steps.attention):
+        return None
+    if steps.post1 is None and steps.post2 is None and steps.scale1 is None and steps.scale2 is None:
+        return None
+    if any(_norm_form(getattr(module, n)) is None for n in (steps.pre1, steps.post1, steps.pre2, steps.post2) if n):
+        return None
+    return steps
+
+
+_NORM_FORMS: dict[type, float | None] = {}
+
+
+def _norm_form(norm: nn.Module) -> float | None:
+    """What is added to a normalisation module's weight (0 or 1) if it is an RMSNorm of the last dimension, found by
+    what its forward does to a small host tensor; None otherwise."""
+    cls = type(norm)
+    if cls not in _NORM_FORMS:
+        import copy
+
+        _NORM_FORMS[cls] = None
+        weight, eps = getattr(norm, "weight", None), _norm_eps(norm)
+        if isinstance(weight, Tensor) and weight.ndim == 1 and eps is not None and not list(norm.children()):
+            gen = torch.Generator().manual_seed(0)
+            x, w = torch.randn(3, 8, generator=gen), torch.randn(8, generator=gen)
+            try:
+                probe = copy.copy(norm)
+                probe._parameters = {"weight": nn.Parameter(w, requires_grad=False)}
+                with torch.no_grad():
+                    got = cls.forward(probe, x)
+                unit = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + eps)
+                for offset in (0.0, 1.0):
+                    if torch.allclose(got, unit * (w + offset), rtol=1e-5, atol=1e-6):
+                        _NORM_FORMS[cls] = offset
+            except Exception:
+                pass
+    return _NORM_FORMS[cls]
+
+
+def _norm_eps(norm: nn.Module) -> float | None:
+    for name in ("variance_epsilon", "eps"):
+        eps = getattr(norm, name, None)
+        if isinstance(eps, float):
+            return eps
+    return None
+
+
+def _between_blocks(x: Tensor, branch: Tensor, post: nn.Module | None, pre: nn.Module | None,
+                    scale: float) -> tuple[Tensor, Tensor]:
+    """(x + scale post(branch), pre of it): one launch where `block_norms` takes the tensors, else step by step."""
+    w1, w2 = (None if n is None else n.weight for n in (post, pre))
+    forms = {_norm_form(n) for n in (post, pre) if n is not None}
+    if len(forms) <= 1 and not any(hasattr(w, "to_local") for w in (w1, w2)) \
+            and block_norms_supported(x, branch, w1, w2):
+        e1 = _norm_eps(post) if post is not None else 0.0
+        hidden, normed = block_norms(x, branch, w1, w2, scale=scale, eps=e1, pre_eps=_norm_eps(pre) if pre is not None else e1,
+                                     weight_offset=forms.pop() if forms else 0.0)
+        return hidden, hidden if normed is None else normed
+    if post is not None:
+        branch = post(branch)
+    hidden = x + (branch if scale == 1.0 else branch * scale)
+    return hidden, hidden if pre is None else pre(hidden)
+
+
+def _fused_steps_forward(self: nn.Module, hidden_states: Tensor, *args: Any, **kwargs: Any) -> Tensor:
+    """The forward of a decoder layer with a norm behind a block or a factor on its branch (`_layer_steps`): what lies
+    between attention and MLP, and behind the MLP, in one launch each."""
+    steps: _LayerSteps = self._prl_steps
+    norm = lambda name: None if name is None else getattr(self, name)
+    bound = steps.signature.bind(self, hidden_states, *args, **kwargs)
+    bound.apply_defaults()
+    x = hidden_states
+    bound.arguments["hidden_states"] = x if steps.pre1 is None else norm(steps.pre1)(x)
+    call: dict[str, Any] = {}
+    for name, value in steps.attention:
+        if name is None:
+            call.update(bound.arguments[value])
+        else:
+            call[name] = bound.arguments[value]
+    branch = self.self_attn(**call)[0]
+    factor = lambda name: 1.0 if name is None else float(getattr(self, name))
+    x, normed = _between_blocks(x, branch, norm(steps.post1), norm(steps.pre2), factor(steps.scale1))
+    return _between_blocks(x, self.mlp(normed), norm(steps.post2), None, factor(steps.scale2))[0]
 
 
 def enable_residual_carry(model: nn.Module, on: bool = True) -> int:
@@ -1169,13 +1417,27 @@ def fuse_model(model: nn.Module) -> dict[str, int]:
     layers_too = os.environ.get("PRL_FUSED_LAYER", "1") != "0"  # the residual additions inside the norm kernels
 
     home = sys.modules.get(type(model).__module__)  # e.g. transformers.models.qwen3.modeling_qwen3
+    kind = None
     if home is not None and hasattr(home, "apply_rotary_pos_emb"):
-        if home.__name__ not in _PATCHED_MODULES:
-            _PATCHED_MODULES[home.__name__] = home.apply_rotary_pos_emb
-            if not _ORIGINAL_ROPE:
-                _ORIGINAL_ROPE.append(home.apply_rotary_pos_emb)
-            home.apply_rotary_pos_emb = apply_rotary_pos_emb  # module-wide: every model of this family in the process
-        done["rope"] = 1
+        if home.__name__ in _PATCHED_MODULES:  # (what the patch replaced is what tells the pairs)
+            patched, home.apply_rotary_pos_emb = home.apply_rotary_pos_emb, _PATCHED_MODULES[home.__name__]
+            kind = _rope_kind(home, model)
+            home.apply_rotary_pos_emb = patched
+        else:
+            kind = _rope_kind(home, model)
+        if kind is not None:
+            if home.__name__ not in _PATCHED_MODULES:
+                _PATCHED_MODULES[home.__name__] = home.apply_rotary_pos_emb
+                if not _ORIGINAL_ROPE:
+                    _ORIGINAL_ROPE.append(home.apply_rotary_pos_emb)
+                # module-wide: every model of this family in the process
+                home.apply_rotary_pos_emb = _family_rope(home.apply_rotary_pos_emb, kind[0])
+            for rotary in kind[1]:
+                if not hasattr(rotary, "_prl_torch_forward"):
+                    rotary._prl_torch_forward = rotary.forward
+                    rotary.forward = types.MethodType(_tagged_rotary_forward, rotary)
+            done["rope"] = 1
+    whole_heads_in_halves = kind is not None and kind[0] == "half" and not kind[1]
     head = getattr(model, "lm_head", None)  # its products on this package's MFMA kernels where they are ahead
     if isinstance(head, nn.Linear) and head.bias is None and not hasattr(head, "_prl_torch_forward"):
         head._prl_torch_forward = head.forward
@@ -1193,6 +1455,13 @@ def fuse_model(model: nn.Module) -> dict[str, int]:
             module._prl_carry, module._prl_first = None, False
             module.forward = types.MethodType(_fused_layer_forward, module)
             done["layer"] += 1
+        elif layers_too and not hasattr(module, "_prl_torch_forward"):
+            steps = _layer_steps(module)
+            if steps is not None:
+                module._prl_torch_forward = module.forward
+                module._prl_steps = steps
+                module.forward = types.MethodType(_fused_steps_forward, module)
+                done["layer"] += 1
         is_gated_mlp = name.endswith("MLP") and all(hasattr(module, a) for a in ("gate_proj", "up_proj", "down_proj")) \
             and type(getattr(module, "act_fn", None)).__name__ in ("SiLU", "SiLUActivation")
         if is_gated_mlp and not hasattr(module, "_prl_torch_forward"):
@@ -1223,7 +1492,8 @@ def fuse_model(model: nn.Module) -> dict[str, int]:
                 m.forward = types.MethodType(fn, m)
             done["qkv"] += 1
             if hasattr(module, "q_norm") and hasattr(module, "k_norm") and hasattr(module, "head_dim") \
-                    and hasattr(module, "o_proj") and not hasattr(module, "_prl_torch_forward"):
+                    and hasattr(module, "o_proj") and not hasattr(module, "_prl_torch_forward") \
+                    and (whole_heads_in_halves or not hasattr(home, "apply_rotary_pos_emb")):
                 module._prl_torch_forward = module.forward
                 module.forward = types.MethodType(_fused_attention_forward, module)
     return done
@@ -1239,7 +1509,7 @@ def unfuse_model(model: nn.Module) -> None:
         if hasattr(module, "_prl_torch_forward"):
             module.forward = module._prl_torch_forward
             del module._prl_torch_forward
-            for attr in ("_prl_qkv", "_prl_carry", "_prl_first"):
+            for attr in ("_prl_qkv", "_prl_carry", "_prl_first", "_prl_steps"):
                 if hasattr(module, attr):
                     delattr(module, attr)
 

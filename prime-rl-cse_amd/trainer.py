@@ -26,6 +26,7 @@ from .batch import host_to_device, to_device
 from .config import LossConfig
 from .data import MicroBatch
 from .loss import policy_loss, unit_gradient
+from .optim import clip_grad_norm_, clip_grad_norm_supported
 from .utils import Tensors
 
 # Literal architecture dimensions (there is no hub access where this runs).  The
@@ -742,7 +743,9 @@ def train_step(model: nn.Module, optimizer: torch.optim.Optimizer, micro_batches
         for prm in model.parameters():
             if prm.requires_grad and prm.grad is None:
                 prm.grad = torch.zeros_like(prm)
-    grad_norm = torch.nn.utils.clip_grad_norm_(model.parameters(), max_norm=max_norm)
+    params = [prm for prm in model.parameters() if prm.grad is not None]
+    clip = clip_grad_norm_ if clip_grad_norm_supported([prm.grad for prm in params]) else torch.nn.utils.clip_grad_norm_
+    grad_norm = clip(params, max_norm)
     if hasattr(grad_norm, "full_tensor"):
         grad_norm = grad_norm.full_tensor()
     optimizer.step()
