@@ -921,25 +921,29 @@ class _Carry:
     while a branch is pending fails instead of computing without it."""
 
     def __init__(self) -> None:
-        self.hidden: Tensor | None = None
-        self.branch: Tensor | None = None
+        self.clear()
 
     def clear(self) -> None:
-        self.hidden = self.branch = None
+        self.hidden: Tensor | None = None
+        self.branch: Tensor | None = None
+        self.behind: tuple[nn.Module | None, float] | None = None  # norm behind the block and factor, if it has any
 
-    def put(self, hidden: Tensor, branch: Tensor) -> None:
-        self.hidden, self.branch = hidden, branch
+    def put(self, hidden: Tensor, branch: Tensor, behind: tuple[nn.Module | None, float] | None = None) -> None:
+        self.hidden, self.branch, self.behind = hidden, branch, behind
 
-    def take(self, hidden: Tensor) -> Tensor | None:
+    def join(self, hidden: Tensor, norm: nn.Module | None) -> tuple[Tensor, Tensor] | None:
+        """(hidden with the pending branch added, `norm` of it), or None if nothing is pending."""
         if self.branch is None:
             return None
-        mine, branch = self.hidden is hidden, self.branch
+        mine, branch, behind = self.hidden is hidden, self.branch, self.behind
         self.clear()
         if not mine:
             raise RuntimeError("fused blocks: the output of a block was replaced before the next block or the final "
                                "norm read it; the residual carry needs them called back to back "
                                "(fused.enable_residual_carry(model, False) switches it off)")
-        return branch
+        if behind is None and norm is not None:
+            return _add_norm(norm, hidden, branch)
+        return _between_blocks(hidden, branch, *(behind or (None, 1.0)), pre=norm)
 
 
 def _add_norm(norm: nn.Module, x: Tensor, branch: Tensor) -> tuple[Tensor, Tensor]:
@@ -959,13 +963,13 @@ def _fused_layer_forward(self: nn.Module, hidden_states: Tensor, attention_mask:
     the MLP when the layers hand it on (`enable_residual_carry`)."""
     carry: _Carry | None = self._prl_carry
     x = hidden_states
-    pending = None
+    joined = None
     if carry is not None:
         if self._prl_first:
             carry.clear()  # nothing of an earlier, abandoned forward
-        pending = carry.take(x)
-    if pending is not None:
-        x, normed = _add_norm(self.input_layernorm, x, pending)
+        joined = carry.join(x, self.input_layernorm)
+    if joined is not None:
+        x, normed = joined
     else:
         normed = self.input_layernorm(x)
     branch, _ = self.self_attn(hidden_states=normed, attention_mask=attention_mask, position_ids=position_ids,
@@ -1140,8 +1144,8 @@ def _norm_eps(norm: nn.Module) -> float | None:
     return None
 
 
-def _between_blocks(x: Tensor, branch: Tensor, post: nn.Module | None, pre: nn.Module | None,
-                    scale: float) -> tuple[Tensor, Tensor]:
+def _between_blocks(x: Tensor, branch: Tensor, post: nn.Module | None, scale: float,
+                    pre: nn.Module | None) -> tuple[Tensor, Tensor]:
     """(x + scale post(branch), pre of it): one launch where `block_norms` takes the tensors, else step by step."""
     w1, w2 = (None if n is None else n.weight for n in (post, pre))
     forms = {_norm_form(n) for n in (post, pre) if n is not None}
@@ -1154,18 +1158,32 @@ def _between_blocks(x: Tensor, branch: Tensor, post: nn.Module | None, pre: nn.M
     if post is not None:
         branch = post(branch)
     hidden = x + (branch if scale == 1.0 else branch * scale)
-    return hidden, hidden if pre is None else pre(hidden)
+    if pre is None:
+        return hidden, hidden
+    plain = getattr(pre, "_prl_torch_forward", pre)  # (the rebound final norm would look for a pending branch)
+    return hidden, plain(hidden)
 
 
 def _fused_steps_forward(self: nn.Module, hidden_states: Tensor, *args: Any, **kwargs: Any) -> Tensor:
     """The forward of a decoder layer with a norm behind a block or a factor on its branch (`_layer_steps`): what lies
-    between attention and MLP, and behind the MLP, in one launch each."""
+    between attention and MLP in one launch, and so behind the MLP, in the next layer's where the layers hand their
+    last branch on (`enable_residual_carry`)."""
     steps: _LayerSteps = self._prl_steps
     norm = lambda name: None if name is None else getattr(self, name)
     bound = steps.signature.bind(self, hidden_states, *args, **kwargs)
     bound.apply_defaults()
     x = hidden_states
-    bound.arguments["hidden_states"] = x if steps.pre1 is None else norm(steps.pre1)(x)
+    carry: _Carry | None = self._prl_carry
+    joined = None
+    if carry is not None:
+        if self._prl_first:
+            carry.clear()
+        joined = carry.join(x, norm(steps.pre1))
+    if joined is not None:
+        x, normed = joined
+    else:
+        normed = x if steps.pre1 is None else norm(steps.pre1)(x)
+    bound.arguments["hidden_states"] = normed
     call: dict[str, Any] = {}
     for name, value in steps.attention:
         if name is None:
@@ -1174,8 +1192,12 @@ def _fused_steps_forward(self: nn.Module, hidden_states: Tensor, *args: Any, **k
             call[name] = bound.arguments[value]
     branch = self.self_attn(**call)[0]
     factor = lambda name: 1.0 if name is None else float(getattr(self, name))
-    x, normed = _between_blocks(x, branch, norm(steps.post1), norm(steps.pre2), factor(steps.scale1))
-    return _between_blocks(x, self.mlp(normed), norm(steps.post2), None, factor(steps.scale2))[0]
+    x, normed = _between_blocks(x, branch, norm(steps.post1), factor(steps.scale1), norm(steps.pre2))
+    branch = self.mlp(normed)
+    if carry is None:
+        return _between_blocks(x, branch, norm(steps.post2), factor(steps.scale2), None)[0]
+    carry.put(x, branch, (norm(steps.post2), factor(steps.scale2)))
+    return x
 
 
 def enable_residual_carry(model: nn.Module, on: bool = True) -> int:
@@ -1204,9 +1226,9 @@ def enable_residual_carry(model: nn.Module, on: bool = True) -> int:
 def _fused_rmsnorm_forward(self: nn.Module, hidden_states: Tensor) -> Tensor:
     carry: _Carry | None = getattr(self, "_prl_carry", None)
     if carry is not None:  # the final norm behind layers that carry their last addition
-        pending = carry.take(hidden_states)
-        if pending is not None:
-            return _add_norm(self, hidden_states, pending)[1]
+        joined = carry.join(hidden_states, self)
+        if joined is not None:
+            return joined[1]
     weight = self.weight
     if hasattr(weight, "to_local"):  # a DTensor outside an FSDP forward: leave it to torch
         return self._prl_torch_forward(hidden_states)
@@ -1460,6 +1482,7 @@ def fuse_model(model: nn.Module) -> dict[str, int]:
             if steps is not None:
                 module._prl_torch_forward = module.forward
                 module._prl_steps = steps
+                module._prl_carry, module._prl_first = None, False
                 module.forward = types.MethodType(_fused_steps_forward, module)
                 done["layer"] += 1
         is_gated_mlp = name.endswith("MLP") and all(hasattr(module, a) for a in ("gate_proj", "up_proj", "down_proj")) \

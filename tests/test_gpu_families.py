@@ -60,6 +60,36 @@ def test_logits_and_gradients_are_those_of_the_unfused_model(name):
     assert torch.equal(again, want)  # everything is as it was
 
 
+@pytest.mark.parametrize("name", ["Glm4", "Olmo2", "Granite"])
+def test_the_last_branch_handed_to_the_next_layer(name):
+    """`enable_residual_carry` over such layers: the norm behind the MLP runs with the next layer's first norm."""
+    model = tiny(name, num_hidden_layers=3, **({"residual_multiplier": 0.22} if name == "Granite" else {})).to(DEV)
+    ids = torch.arange(40, device=DEV)[None] % 160
+    pos = torch.arange(40, device=DEV)[None]
+    weights = torch.randn(1, 40, 160, generator=torch.Generator(device=DEV).manual_seed(4), device=DEV)
+    want, wgrads = run(model, ids, pos, weights)
+    fused.fuse_model(model)
+    try:
+        assert fused.enable_residual_carry(model) == 3
+        timer = prl._capi.KernelTimer()
+        prl._capi.set_timer(timer)
+        got, grads = run(model, ids, pos, weights)
+        prl._capi.set_timer(None)
+        seen = timer.summary()
+        # nothing of a layer's norms is left to the norm kernels but the first layer's own (if it has one)
+        assert seen["prl_block_norms_fwd"]["launches"] == 6
+        assert seen.get("prl_rmsnorm_fwd", {"launches": 0})["launches"] <= 1 + 2 * 3  # (query / key norms)
+        assert fused.enable_residual_carry(model, False) == 0
+        assert (T.forward(model, ids, pos) - want).abs().max() <= 2000 * 2.0**-24 * want.abs().max()
+    finally:
+        prl._capi.set_timer(None)
+        fused.unfuse_model(model)
+    assert not hasattr(model.model.layers[0], "_prl_carry")
+    assert (got - want).abs().max() <= 2000 * 2.0**-24 * want.abs().max()
+    for n, g in grads.items():
+        assert (g - wgrads[n]).norm() <= 2000 * 2.0**-24 * wgrads[n].norm() + 1e-12, n
+
+
 def test_two_families_in_one_process_keep_their_own_pairs():
     first, second = tiny("Qwen3").to(DEV), tiny("Glm4").to(DEV)
     ids, pos = torch.arange(32, device=DEV)[None], torch.arange(32, device=DEV)[None]
