@@ -15,6 +15,7 @@ moves to the host).
 
 from __future__ import annotations
 
+import functools
 import types
 from typing import Any
 
@@ -353,7 +354,14 @@ def block_norms(x: Tensor, branch: Tensor, post_weight: Tensor | None = None, pr
 
 
 def _strides6(x: Tensor, out: Tensor):
-    return (C.c_int64 * 6)(x.stride(0), x.stride(1), x.stride(2), out.stride(0), out.stride(1), out.stride(2))
+    return _stride_array(x.stride()[:3], out.stride()[:3])
+
+
+@functools.lru_cache(maxsize=1024)
+def _stride_array(x: tuple[int, int, int], out: tuple[int, int, int]):
+    """The HOST array of six strides the library reads (never writes); building one costs 0.9 us of host time, three
+    times that in the autograd engine's thread."""
+    return (C.c_int64 * 6)(*x, *out)
 
 
 def _launch_rope(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, inverse: bool) -> tuple[Tensor, Tensor]:
