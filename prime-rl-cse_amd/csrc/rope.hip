@@ -98,16 +98,16 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope_positions(RopeSide q, Rop
                                                                  RopeShape sh, const char* __restrict__ pos, int pos64,
                                                                  int64_t pos_b, int64_t pos_t,
                                                                  const char* __restrict__ inv_freq, int freq64,
-                                                                 float amplitude, int inverse, int n_tokens, int T) {
+                                                                 float amplitude, int inverse, int first, int n_tokens, int T) {
   using P = RopeUnit<DT, VEC>;
   constexpr int N = P::kN, ES = P::kEs;
   extern __shared__ float2 cs[];  // [token of the workgroup][pair]
   const int half = sh.r >> 1;
-  const int tok0 = blockIdx.x * sh.toks;
+  const int tok0 = first + blockIdx.x * sh.toks;
   const int ntok = min(sh.toks, n_tokens - tok0);
   for (int i = threadIdx.x; i < ntok * half; i += kRopeThreads) {
-    const int tok = i / half, j = i - tok * half;
-    const int n = tok0 + tok, b = n / T, t = n - b * T;
+    const int tk = i / half, j = i - tk * half;
+    const int n = tok0 + tk, b = n / T, t = n - b * T;
     const char* pp = pos + b * pos_b + t * pos_t;
     const double p = pos64 ? (double)*reinterpret_cast<const int64_t*>(pp) : (double)*reinterpret_cast<const int32_t*>(pp);
     const double f = freq64 ? reinterpret_cast<const double*>(inv_freq)[j] : (double)reinterpret_cast<const float*>(inv_freq)[j];
@@ -237,19 +237,22 @@ extern "C" int prl_rope_positions(const void* q, void* q_out, const int64_t* q_s
   const bool vec = ((bits | (uintptr_t)(D * es) | (uintptr_t)(interleaved ? 0 : half * es)) & 15) == 0;
   const int64_t tokens = B * T;
   const RopeShape sh = rope_shape(rotary_dim, D, heads, ve, interleaved, vec);
-  const int64_t grid = (tokens + sh.toks - 1) / sh.toks;
   const size_t lds = (size_t)sh.toks * half * sizeof(float2);
 #define PRL_ROPE(DT, IL, VEC)                                                                                       \
-  hipLaunchKernelGGL((k_rope_positions<DT, IL, VEC>), dim3((unsigned)grid), dim3(kRopeThreads), lds, (hipStream_t)stream, \
+  hipLaunchKernelGGL((k_rope_positions<DT, IL, VEC>), dim3(grid), dim3(kRopeThreads), lds, (hipStream_t)stream, \
                      side[0], side[1], (int)q_heads, (int)heads, sh, (const char*)positions, positions_64 ? 1 : 0,   \
                      pos_batch_stride * (positions_64 ? 8 : 4), pos_token_stride * (positions_64 ? 8 : 4),           \
-                     (const char*)inv_freq, inv_freq_64 ? 1 : 0, amplitude, inverse ? 1 : 0, (int)tokens, (int)T)
+                     (const char*)inv_freq, inv_freq_64 ? 1 : 0, amplitude, inverse ? 1 : 0, (int)first, (int)tokens, (int)T)
 #define PRL_ROPE_VEC(DT, IL) \
   if (vec) PRL_ROPE(DT, IL, true); else PRL_ROPE(DT, IL, false)
-  if (dtype == PRL_BF16) {
-    if (interleaved) { PRL_ROPE_VEC(PRL_BF16, true); } else { PRL_ROPE_VEC(PRL_BF16, false); }
-  } else {
-    if (interleaved) { PRL_ROPE_VEC(PRL_F32, true); } else { PRL_ROPE_VEC(PRL_F32, false); }
+  const int64_t most = (int64_t)sh.toks << 22;  // tokens of a launch, which holds fewer than 2^32 threads
+  for (int64_t first = 0; first < tokens; first += most) {
+    const unsigned grid = (unsigned)(((tokens - first < most ? tokens - first : most) + sh.toks - 1) / sh.toks);
+    if (dtype == PRL_BF16) {
+      if (interleaved) { PRL_ROPE_VEC(PRL_BF16, true); } else { PRL_ROPE_VEC(PRL_BF16, false); }
+    } else {
+      if (interleaved) { PRL_ROPE_VEC(PRL_F32, true); } else { PRL_ROPE_VEC(PRL_F32, false); }
+    }
   }
 #undef PRL_ROPE_VEC
 #undef PRL_ROPE

@@ -439,6 +439,8 @@ def _tagged_rotary_forward(self: nn.Module, x: Tensor, position_ids: Tensor, *ar
     """A rotary module's own forward, with its positions and frequencies left on the cos it returns for the attention
     blocks' rotary function (`_family_rope`), which gets that very tensor."""
     cos, sin = self._prl_torch_forward(x, position_ids, *args, **kwargs)
+    if args or kwargs:  # a module with several sets of frequencies: which one these came from is its own business
+        return cos, sin
     inv_freq = self.inv_freq  # (read after the call: frequencies that depend on the length are set in there)
     if inv_freq.dtype != torch.float32:
         inv_freq = inv_freq.float()  # as the module itself uses it

@@ -151,9 +151,9 @@ def clip_grad_norm_supported(grads: list[torch.Tensor]) -> bool:
     if _sharding(grads) is None:
         return False
     parts = _local_parts(grads)
-    dev = parts[0].device
-    return dev.type == "cuda" and all(g.layout == torch.strided and g.device == dev and _is_one_run(g)
-                                      and g.dtype in (torch.float32, torch.bfloat16) for g in parts)
+    index = set(map(torch.Tensor.get_device, parts))
+    return len(index) == 1 and index != {-1} and set(map(_DTYPE, parts)) <= _TYPES \
+        and all(g.layout is torch.strided and _is_one_run(g) for g in parts)
 
 
 _GRAD, _DTYPE = operator.attrgetter("grad"), operator.attrgetter("dtype")

@@ -206,3 +206,29 @@ def test_captured_and_replayed_and_on_other_streams():
         b = run()
     torch.cuda.synchronize()
     assert torch.equal(a[0], want[0]) and torch.equal(b[0], want[0])
+
+
+def test_heads_that_are_one_head_expanded():
+    q, k = inputs(2, 21, 1, 1, 64, torch.bfloat16, "bthd")
+    pos = torch.arange(21, device=DEV)
+    f, _ = fused.rope_frequencies(64, device=DEV)
+    k.requires_grad_(True)
+    qo, ko = fused.rope_at_positions(q, k.expand(2, 6, 21, 64), pos, f)
+    one = fused.rope_at_positions(q, k.detach(), pos, f)[1]
+    assert torch.equal(ko, one.expand(2, 6, 21, 64))
+    g = torch.randn(2, 6, 21, 64, device=DEV).bfloat16()
+    ko.backward(g)  # the heads' gradients are added up
+    theta = (pos.double()[:, None] * f.double())[None, None]
+    want, m = turned(g, -theta, 1.0, 64, False)
+    tol = (m * 6e-7 + 2.0**-8 * want.abs()).sum(1, keepdim=True) + 2.0**-8 * want.sum(1, keepdim=True).abs() + 6 * 2.0**-23
+    assert bool(((k.grad.double() - want.sum(1, keepdim=True)).abs() <= tol).all())
+
+
+def test_more_tokens_than_a_launch_has_workgroups_for():
+    n = (1 << 23) + 12345  # two tokens a workgroup, 2^22 workgroups
+    x = torch.randn(1, 1, n, 2, device=DEV)
+    pos = torch.arange(n, device=DEV)
+    f = torch.ones(1, device=DEV)
+    out, _ = fused.rope_at_positions(x, None, pos, f)
+    for cut in (slice(0, 1000), slice((1 << 23) - 1000, n)):
+        check(out[:, :, cut], x[:, :, cut], pos[cut].double()[None, None, :, None], 1.0, 2, False)
