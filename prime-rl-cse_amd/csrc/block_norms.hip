@@ -24,25 +24,29 @@
 namespace prl {
 
 constexpr int kBnMaxH = 8192;
+enum { kBnElems = 0, kBnVec = 1, kBnStream = 2 };  // single elements; vectors; vectors past the caches
 constexpr int kBnRsrcFlags = 0x00020000;  // raw buffer, 32-bit data format (gfx9 family descriptor word 3)
 
-// A thread reads its share of a row in units of four registers.  VEC: a unit is 16 consecutive bytes, unit v at
+// A thread reads its share of a row in units of four registers.  In the vector modes a unit is 16 consecutive bytes, unit v at
 // 16 v, for rows whose every unit is whole and aligned.  Otherwise it is four single elements, `tpr` apart, so that a
 // wave's accesses lie side by side whatever the row's alignment: 16-byte accesses at odd places ran at half the
 // rate (8192 rows of 1531 bf16, a gate per element: forward 45.0 us against 31.8, backward 82.6 against 53.4).
 // Rows are read through descriptors of exactly their bytes: lanes beyond the end, and every lane of a tensor that is
 // not there, read 0 and store nothing, without a branch.
-template <int DT, bool VEC>
+template <int DT, int MODE>
 struct BnUnit {
+  static constexpr bool VEC = MODE != kBnElems;
+  static constexpr int kAux = MODE == kBnStream ? 2 : 0;  // non-temporal
   static constexpr int kEs = DT == PRL_F32 ? 4 : 2;
   static constexpr int kN = VEC ? 16 / kEs : 4;  // elements
   // column of element i of unit k of thread li
   static __device__ __forceinline__ int column(int k, int i, int li, int tpr) {
     return VEC ? (li + k * tpr) * kN + i : li + (k * kN + i) * tpr;
   }
+  template <int AUX = kAux>
   static __device__ __forceinline__ u32x4 load(const char* row, int k, int li, int tpr, int H) {
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(row), 0, row ? H * kEs : 0, kBnRsrcFlags);
-    if constexpr (VEC) return __builtin_amdgcn_raw_buffer_load_b128(rsrc, (li + k * tpr) * 16, 0, 0);
+    if constexpr (VEC) return __builtin_amdgcn_raw_buffer_load_b128(rsrc, (li + k * tpr) * 16, 0, AUX);
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -70,7 +74,7 @@ struct BnUnit {
       } else {
         z.x = pack_bf16(y[0], y[1]), z.y = pack_bf16(y[2], y[3]), z.z = pack_bf16(y[4], y[5]), z.w = pack_bf16(y[6], y[7]);
       }
-      __builtin_amdgcn_raw_buffer_store_b128(z, rsrc, (li + k * tpr) * 16, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b128(z, rsrc, (li + k * tpr) * 16, 0, kAux);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -161,9 +165,9 @@ struct BnIn {
   int gate_kind;
 };
 
-template <int DT, int NV, bool BWD, int GATE, bool VEC>
+template <int DT, int NV, bool BWD, int GATE, int MODE>
 __device__ __forceinline__ void bn_fetch(BnRow<NV, BWD, GATE>& r, const BnIn& in, int64_t row, int li, int tpr, int H) {
-  using U = BnUnit<DT, VEC>;
+  using U = BnUnit<DT, MODE>;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     r.b[k] = U::load(in.b.row(row), k, li, tpr, H);
@@ -178,16 +182,16 @@ __device__ __forceinline__ void bn_fetch(BnRow<NV, BWD, GATE>& r, const BnIn& in
 }
 
 // What a thread reads once: its columns of the weights and of a gate per channel.
-template <int DT, int NV, int GATE, bool VEC>
+template <int DT, int NV, int GATE, int MODE>
 struct BnCols {
-  using U = BnUnit<DT, VEC>;
+  using U = BnUnit<DT, MODE>;
   u32x4 w1[NV], w2[NV], g[GATE ? NV : 1];
   __device__ __forceinline__ void load(const BnIn& in, int li, int tpr, int H) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      w1[k] = U::load(in.w1, k, li, tpr, H);
-      w2[k] = U::load(in.w2, k, li, tpr, H);
-      if (GATE == 1) g[k] = U::load(in.gate.p, k, li, tpr, H);
+      w1[k] = U::template load<0>(in.w1, k, li, tpr, H);
+      w2[k] = U::template load<0>(in.w2, k, li, tpr, H);
+      if (GATE == 1) g[k] = U::template load<0>(in.gate.p, k, li, tpr, H);
     }
   }
   // Keeps them packed through the loop over rows: the compiler would unpack what does not change in front of it, into
@@ -206,12 +210,12 @@ struct BnCols {
 
 // ONEWAVE: a wave per row, blockDim / 64 rows at a time; otherwise a workgroup per row.  The next row's loads go out
 // as soon as this one's are unpacked and stay in flight while it is worked on.  BOTH: both weights are there.
-template <int DT, int NV, bool ONEWAVE, int GATE, bool VEC, bool BOTH>
+template <int DT, int NV, bool ONEWAVE, int GATE, int MODE, bool BOTH>
 __global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_fwd(BnIn in, float scale, float offset, float eps1,
                                                                           float eps2, BnRowsOut h, BnRowsOut y,
                                                                           float* __restrict__ rstd1,
                                                                           float* __restrict__ rstd2, int64_t rows, int H) {
-  using U = BnUnit<DT, VEC>;
+  using U = BnUnit<DT, MODE>;
   constexpr int VE = U::kN;
   const bool has1 = BOTH || in.w1 != nullptr, has2 = BOTH || in.w2 != nullptr;
   __shared__ float slots[2][16];
@@ -222,9 +226,9 @@ __global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_fwd(BnIn i
   int64_t row = (int64_t)blockIdx.x * (ONEWAVE ? blockDim.x >> 6 : 1) +
                 (ONEWAVE ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
   if (row >= rows) return;
-  BnCols<DT, NV, GATE, VEC> w;
+  BnCols<DT, NV, GATE, MODE> w;
   BnRow<NV, false, GATE> cur;
-  bn_fetch<DT, NV, false, GATE, VEC>(cur, in, row, li, tpr, H);
+  bn_fetch<DT, NV, false, GATE, MODE>(cur, in, row, li, tpr, H);
   w.load(in, li, tpr, H);
   for (;;) {
     const int64_t next = row + step;
@@ -243,7 +247,7 @@ __global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_fwd(BnIn i
       for (int i = 0; i < VE; ++i) ss = fmaf(bv[k][i], bv[k][i], ss);
     }
     const float gt = cur.gt;
-    if (next < rows) bn_fetch<DT, NV, false, GATE, VEC>(cur, in, next, li, tpr, H);
+    if (next < rows) bn_fetch<DT, NV, false, GATE, MODE>(cur, in, next, li, tpr, H);
     float r1 = 1.0f;
     if (has1) {
       r1 = rsqrtf(bn_row_sum<ONEWAVE>(ss, slots[0]) * inv_h + eps1);
@@ -293,13 +297,13 @@ __global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_fwd(BnIn i
 
 // part[array][blockIdx.x][H]: arrays 0 gw1, 1 gw2, 2 a channel gate's gradient (for a gate of one value: [blockIdx.x]),
 // each there only when asked for
-template <int DT, int NV, bool ONEWAVE, int GATE, bool VEC, bool BOTH>
+template <int DT, int NV, bool ONEWAVE, int GATE, int MODE, bool BOTH>
 __global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_bwd(BnIn in, float scale, float offset, BnRowsOut gx,
                                                                           BnRowsOut gb, float* __restrict__ part1,
                                                                           float* __restrict__ part2,
                                                                           float* __restrict__ partg, BnRowsOut gg,
                                                                           int64_t rows, int H) {
-  using U = BnUnit<DT, VEC>;
+  using U = BnUnit<DT, MODE>;
   constexpr int VE = U::kN;
   const bool has1 = BOTH || in.w1 != nullptr, has2 = BOTH || in.w2 != nullptr;
   __shared__ float slots[3][16];
@@ -316,9 +320,9 @@ __global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_bwd(BnIn i
 #pragma unroll
     for (int i = 0; i < VE; ++i) a1[k][i] = a2[k][i] = ag[GATE == 1 ? k : 0][i] = 0.0f;
   int64_t row = (int64_t)blockIdx.x * rpb + slot;
-  BnCols<DT, NV, GATE, VEC> w;
+  BnCols<DT, NV, GATE, MODE> w;
   BnRow<NV, true, GATE> cur;
-  if (row < rows) bn_fetch<DT, NV, true, GATE, VEC>(cur, in, row, li, tpr, H);
+  if (row < rows) bn_fetch<DT, NV, true, GATE, MODE>(cur, in, row, li, tpr, H);
   w.load(in, li, tpr, H);
   while (row < rows) {
     const int64_t next = row + step;
@@ -360,7 +364,7 @@ __global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_bwd(BnIn i
         }
       }
     }
-    if (next < rows) bn_fetch<DT, NV, true, GATE, VEC>(cur, in, next, li, tpr, H);
+    if (next < rows) bn_fetch<DT, NV, true, GATE, MODE>(cur, in, next, li, tpr, H);
     if (has2) dot = bn_row_sum<ONEWAVE>(dot, slots[0]) * inv_h;
     float dot1 = 0.0f, gdot = 0.0f;
 #pragma unroll
@@ -425,10 +429,10 @@ __global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_bwd(BnIn i
     for (int k = 0; k < NV; ++k) {
       const float* z = a == 0 ? a1[k] : a == 1 ? a2[k] : ag[GATE == 1 ? k : 0];
 #pragma unroll
-      for (int i = 0; i < VE; i += VEC ? 4 : 1) {
+      for (int i = 0; i < VE; i += U::VEC ? 4 : 1) {
         const int c = U::column(k, i, li, tpr);
         if (c >= H) continue;
-        if (VEC) *reinterpret_cast<float4*>(mine + c) = make_float4(z[i], z[i + 1], z[i + 2], z[i + 3]);
+        if (U::VEC) *reinterpret_cast<float4*>(mine + c) = make_float4(z[i], z[i + 1], z[i + 2], z[i + 3]);
         else mine[c] = z[i];
       }
     }
@@ -552,34 +556,46 @@ static int bn_check(const char* who, int dtype, int64_t rows, int64_t H, int gat
   return PRL_OK;
 }
 
-#define PRL_BN_GATE(KERNEL, DT, NV, OW, VEC, BOTH)                                      \
+#define PRL_BN_GATE(KERNEL, DT, NV, OW, MODE, BOTH)                                     \
   do {                                                                                  \
-    if (gate_kind == PRL_GATE_FULL) KERNEL(DT, NV, OW, 2, VEC, BOTH);                   \
-    else if (gate_kind == PRL_GATE_CHANNEL) KERNEL(DT, NV, OW, 1, VEC, BOTH);           \
-    else KERNEL(DT, NV, OW, 0, VEC, BOTH);                                              \
+    if (gate_kind == PRL_GATE_FULL) KERNEL(DT, NV, OW, 2, MODE, BOTH);                  \
+    else if (gate_kind == PRL_GATE_CHANNEL) KERNEL(DT, NV, OW, 1, MODE, BOTH);          \
+    else KERNEL(DT, NV, OW, 0, MODE, BOTH);                                             \
   } while (0)
-#define PRL_BN_VEC(KERNEL, DT, NV, OW, VEC)                            \
-  do {                                                                 \
-    if (w_post && w_pre) PRL_BN_GATE(KERNEL, DT, NV, OW, VEC, true);   \
-    else PRL_BN_GATE(KERNEL, DT, NV, OW, VEC, false);                  \
+// (the streaming form only with both weights)
+#define PRL_BN_MODE(KERNEL, DT, NV, OW)                                            \
+  do {                                                                             \
+    const bool both = w_post && w_pre;                                             \
+    if (vec && both && stream_past) PRL_BN_GATE(KERNEL, DT, NV, OW, kBnStream, true); \
+    else if (vec && both) PRL_BN_GATE(KERNEL, DT, NV, OW, kBnVec, true);           \
+    else if (vec) PRL_BN_GATE(KERNEL, DT, NV, OW, kBnVec, false);                  \
+    else if (both) PRL_BN_GATE(KERNEL, DT, NV, OW, kBnElems, true);                \
+    else PRL_BN_GATE(KERNEL, DT, NV, OW, kBnElems, false);                         \
   } while (0)
-#define PRL_BN_SHAPE(KERNEL, DT, VEC)                                   \
-  do {                                                                  \
-    if (sh.onewave && sh.nv == 1) PRL_BN_VEC(KERNEL, DT, 1, true, VEC); \
-    else if (sh.onewave) PRL_BN_VEC(KERNEL, DT, 2, true, VEC);          \
-    else PRL_BN_VEC(KERNEL, DT, 1, false, VEC);                         \
+#define PRL_BN_ELEMS(KERNEL, DT, NV, OW)                                     \
+  do {                                                                       \
+    if (w_post && w_pre) PRL_BN_GATE(KERNEL, DT, NV, OW, kBnElems, true);    \
+    else PRL_BN_GATE(KERNEL, DT, NV, OW, kBnElems, false);                   \
   } while (0)
 #define PRL_BN_DISPATCH(KERNEL)                                                           \
   do { /* (two units a thread of a workgroup: rows of more than 4096 fp32 or single elements) */ \
     const bool wide = !sh.onewave && sh.nv == 2;                                          \
-    if (dtype == PRL_F32 && vec && wide) PRL_BN_VEC(KERNEL, PRL_F32, 2, false, true);     \
-    else if (dtype == PRL_F32 && vec) PRL_BN_SHAPE(KERNEL, PRL_F32, true);                \
-    else if (dtype == PRL_F32 && wide) PRL_BN_VEC(KERNEL, PRL_F32, 2, false, false);      \
-    else if (dtype == PRL_F32) PRL_BN_SHAPE(KERNEL, PRL_F32, false);                      \
-    else if (vec) PRL_BN_SHAPE(KERNEL, PRL_BF16, true);                                   \
-    else if (wide) PRL_BN_VEC(KERNEL, PRL_BF16, 2, false, false);                         \
-    else PRL_BN_SHAPE(KERNEL, PRL_BF16, false);                                           \
+    if (dtype == PRL_F32) {                                                               \
+      if (wide) PRL_BN_MODE(KERNEL, PRL_F32, 2, false);                                   \
+      else if (!sh.onewave) PRL_BN_MODE(KERNEL, PRL_F32, 1, false);                       \
+      else if (sh.nv == 1) PRL_BN_MODE(KERNEL, PRL_F32, 1, true);                         \
+      else PRL_BN_MODE(KERNEL, PRL_F32, 2, true);                                         \
+    } else {                                                                              \
+      if (wide) PRL_BN_ELEMS(KERNEL, PRL_BF16, 2, false);                                 \
+      else if (!sh.onewave) PRL_BN_MODE(KERNEL, PRL_BF16, 1, false);                      \
+      else if (sh.nv == 1) PRL_BN_MODE(KERNEL, PRL_BF16, 1, true);                        \
+      else PRL_BN_MODE(KERNEL, PRL_BF16, 2, true);                                        \
+    }                                                                                     \
   } while (0)
+
+// Past the caches from 64 MB on, which would not stay there for the next kernel either (8192 rows of 5120 bf16, forward 64
+// -> 60 us, backward 100 -> 95).
+static bool bn_stream_past(int64_t tensors, int64_t rows, int64_t H, int64_t es) { return tensors * rows * H * es >= (64 << 20); }
 
 extern "C" int prl_block_norms_fwd(const void* x, int64_t x_stride, const void* branch, int64_t branch_stride,
                                    const void* w_post, const void* w_pre, int gate_kind, const void* gate,
@@ -605,8 +621,9 @@ extern "C" int prl_block_norms_fwd(const void* x, int64_t x_stride, const void* 
   const dim3 grid((unsigned)bn_fwd_blocks(rows, sh)), block((unsigned)sh.threads);
   const BnIn in = {{(const char*)x, x_stride * es}, {(const char*)branch, branch_stride * es}, {nullptr, 0}, {nullptr, 0},
                    {(const char*)gate, gate_pitch}, nullptr, nullptr, (const char*)w_post, (const char*)w_pre, gate_kind};
-#define PRL_BN_FWD(DT, NV, OW, GATE, VEC, BOTH)                                                                       \
-  hipLaunchKernelGGL((k_block_norms_fwd<DT, NV, OW, GATE, VEC, BOTH>), grid, block, 0, (hipStream_t)stream, in, scale, \
+  const bool stream_past = bn_stream_past(4, rows, H, es);
+#define PRL_BN_FWD(DT, NV, OW, GATE, MODE, BOTH)                                                                       \
+  hipLaunchKernelGGL((k_block_norms_fwd<DT, NV, OW, GATE, MODE, BOTH>), grid, block, 0, (hipStream_t)stream, in, scale, \
                      weight_offset, eps_post, eps_pre, (BnRowsOut{(char*)hidden, hidden_stride * es}),                \
                      (BnRowsOut{(char*)normed, n_stride * es}), w_post ? rstd_post : nullptr,                         \
                      w_pre ? rstd_pre : nullptr, rows, (int)H)
@@ -670,8 +687,9 @@ extern "C" int prl_block_norms_bwd(const void* x, int64_t x_stride, const void* 
                    (const char*)w_post,
                    (const char*)w_pre,
                    gate_kind};
-#define PRL_BN_BWD(DT, NV, OW, GATE, VEC, BOTH)                                                                       \
-  hipLaunchKernelGGL((k_block_norms_bwd<DT, NV, OW, GATE, VEC, BOTH>), grid, block, lds, st, in, scale, weight_offset, \
+  const bool stream_past = bn_stream_past(6, rows, H, es);
+#define PRL_BN_BWD(DT, NV, OW, GATE, MODE, BOTH)                                                                       \
+  hipLaunchKernelGGL((k_block_norms_bwd<DT, NV, OW, GATE, MODE, BOTH>), grid, block, lds, st, in, scale, weight_offset, \
                      (BnRowsOut{(char*)gx, gx_stride * es}), (BnRowsOut{(char*)g_branch, g_branch_stride * es}), p1, p2, \
                      pg, (BnRowsOut{gg, g_gate_stride * es}), rows, (int)H)
   PRL_BN_DISPATCH(PRL_BN_BWD);

@@ -40,13 +40,14 @@ struct RopeSide {
 // VEC: a thread's two pieces of a head are 16-byte vectors (rows aligned, the pairs of the half layout in whole vectors);
 // otherwise single elements, side by side over the lanes (r = 34 of 128 in the half layout:
 // 53.5 us; 16-byte accesses at places aligned to an element only took 107).
-template <int DT, bool VEC>
+template <int DT, bool VEC, bool NT>
 struct RopeUnit {
   static constexpr int kEs = DT == PRL_F32 ? 4 : 2;
   static constexpr int kN = VEC ? 16 / kEs : 1;  // elements of a piece
   u32x4 z;
   __device__ __forceinline__ void load(const char* p) {
-    if constexpr (VEC) z = *reinterpret_cast<const u32x4*>(p);
+    if constexpr (VEC && NT) z = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+    else if constexpr (VEC) z = *reinterpret_cast<const u32x4*>(p);
     else if constexpr (DT == PRL_F32) z.x = *reinterpret_cast<const uint32_t*>(p);
     else z.x = *reinterpret_cast<const uint16_t*>(p);
   }
@@ -55,7 +56,8 @@ struct RopeUnit {
     else y[0] = DT == PRL_F32 ? __uint_as_float(z.x) : bf16_lo(z.x);
   }
   __device__ __forceinline__ void store(char* p) const {
-    if constexpr (VEC) *reinterpret_cast<u32x4*>(p) = z;
+    if constexpr (VEC && NT) __builtin_nontemporal_store(z, reinterpret_cast<u32x4*>(p));
+    else if constexpr (VEC) *reinterpret_cast<u32x4*>(p) = z;
     else if constexpr (DT == PRL_F32) *reinterpret_cast<uint32_t*>(p) = z.x;
     else *reinterpret_cast<uint16_t*>(p) = (uint16_t)z.x;
   }
@@ -76,10 +78,10 @@ struct RopeShape {
 };
 
 // Turns the two pieces of one head in place; `turn` bit e: pair e belongs to the rotated part.
-template <int DT, bool IL, bool VEC>
-__device__ __forceinline__ void rope_turn(RopeUnit<DT, VEC>& p1, RopeUnit<DT, VEC>& p2, const float* c, const float* s,
+template <int DT, bool IL, bool VEC, bool NT>
+__device__ __forceinline__ void rope_turn(RopeUnit<DT, VEC, NT>& p1, RopeUnit<DT, VEC, NT>& p2, const float* c, const float* s,
                                           uint32_t turn) {
-  constexpr int N = RopeUnit<DT, VEC>::kN;
+  constexpr int N = RopeUnit<DT, VEC, NT>::kN;
   if (!turn) return;
   float x[2 * N], y[2 * N];
   p1.get(x), p2.get(x + N);
@@ -93,13 +95,13 @@ __device__ __forceinline__ void rope_turn(RopeUnit<DT, VEC>& p1, RopeUnit<DT, VE
   p1.put(y), p2.put(y + N);
 }
 
-template <int DT, bool IL, bool VEC>
+template <int DT, bool IL, bool VEC, bool NT>
 __global__ __launch_bounds__(kRopeThreads) void k_rope_positions(RopeSide q, RopeSide k, int q_heads, int heads,
                                                                  RopeShape sh, const char* __restrict__ pos, int pos64,
                                                                  int64_t pos_b, int64_t pos_t,
                                                                  const char* __restrict__ inv_freq, int freq64,
                                                                  float amplitude, int inverse, int first, int n_tokens, int T) {
-  using P = RopeUnit<DT, VEC>;
+  using P = RopeUnit<DT, VEC, NT>;
   constexpr int N = P::kN, ES = P::kEs;
   extern __shared__ float2 cs[];  // [token of the workgroup][pair]
   const int half = sh.r >> 1;
@@ -122,25 +124,29 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope_positions(RopeSide q, Rop
   const int n = tok0 + tok;
   const int64_t b = n / T, t = n - b * T;
   for (int u = u0; u < sh.units; u += sh.per_row) {
-    // the two pieces' first elements, and which of their pairs turn
-    int e1, e2, pair;
+    // The two pieces' first elements, and which of their pairs turn.  Neighbouring lanes take neighbouring pieces.
+    int e1, e2, pair1, pair2;
     uint32_t turn;
-    if (IL) {
-      e1 = 2 * N * u, e2 = e1 + N, pair = N * u;
-      const int on = half - pair;
-      turn = on >= N ? (1u << N) - 1 : on > 0 ? (1u << on) - 1 : 0;
+    if (IL && VEC) {  // half of a unit's pairs in either piece
+      e1 = N * u, e2 = N * (u + sh.units), pair1 = e1 / 2, pair2 = e2 / 2;
+      const int on1 = min(max(half - pair1, 0), N / 2), on2 = min(max(half - pair2, 0), N / 2);
+      turn = ((1u << on1) - 1) | ((1u << on2) - 1) << (N / 2);
+    } else if (IL) {
+      e1 = 2 * u, e2 = e1 + 1, pair1 = pair2 = u;
+      turn = u < half;
     } else {
       const int rot = half / N;
-      pair = N * u;
+      pair1 = pair2 = N * u;
       turn = u < rot;
-      e1 = turn ? pair : sh.r + 2 * N * (u - rot), e2 = turn ? half + pair : e1 + N;
+      e1 = turn ? pair1 : sh.r + N * (u - rot), e2 = turn ? half + pair1 : e1 + N * (sh.units - rot);
     }
     const bool two = e2 < sh.D;
     float c[N], s[N];
     if (turn) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const float2 z = cs[tok * half + (IL ? min(pair + e, half - 1) : pair + e)];
+        const int j = IL && VEC ? min(e < N / 2 ? pair1 + e : pair2 + e - N / 2, half - 1) : pair1 + e;
+        const float2 z = cs[tok * half + j];
         c[e] = z.x, s[e] = z.y;
       }
     }
@@ -161,11 +167,11 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope_positions(RopeSide q, Rop
       P a1, a2, b1, b2;
       a1.load(xa), a2.load(xa + gap);
       if (also) b1.load(xb), b2.load(xb + gap);
-      rope_turn<DT, IL, VEC>(a1, a2, c, s, turn);
+      rope_turn<DT, IL, VEC, NT>(a1, a2, c, s, turn);
       a1.store(oa);
       if (two) a2.store(oa + gap);
       if (also) {
-        rope_turn<DT, IL, VEC>(b1, b2, c, s, turn);
+        rope_turn<DT, IL, VEC, NT>(b1, b2, c, s, turn);
         b1.store(ob);
         if (two) b2.store(ob + gap);
       }
@@ -236,15 +242,19 @@ extern "C" int prl_rope_positions(const void* q, void* q_out, const int64_t* q_s
   // every 16-byte access of a row starts a multiple of 16 bytes from the row's start
   const bool vec = ((bits | (uintptr_t)(D * es) | (uintptr_t)(interleaved ? 0 : half * es)) & 15) == 0;
   const int64_t tokens = B * T;
+  // Past the caches where what is moved would not stay there and a wave's accesses are whole lines (201 MB: 36.6 us
+  // against 41.0; 25 MB: 6.9 against 6.7; 201 MB with 32 of 128 dimensions turned in halves, where a row's pieces lie
+  // scattered: 43.6 against 40.3).
+  const bool nt = 2 * tokens * heads * D * es >= (64 << 20) && (interleaved || rotary_dim == D);
   const RopeShape sh = rope_shape(rotary_dim, D, heads, ve, interleaved, vec);
   const size_t lds = (size_t)sh.toks * half * sizeof(float2);
-#define PRL_ROPE(DT, IL, VEC)                                                                                       \
-  hipLaunchKernelGGL((k_rope_positions<DT, IL, VEC>), dim3(grid), dim3(kRopeThreads), lds, (hipStream_t)stream, \
+#define PRL_ROPE(DT, IL, VEC, NT)                                                                                       \
+  hipLaunchKernelGGL((k_rope_positions<DT, IL, VEC, NT>), dim3(grid), dim3(kRopeThreads), lds, (hipStream_t)stream, \
                      side[0], side[1], (int)q_heads, (int)heads, sh, (const char*)positions, positions_64 ? 1 : 0,   \
                      pos_batch_stride * (positions_64 ? 8 : 4), pos_token_stride * (positions_64 ? 8 : 4),           \
                      (const char*)inv_freq, inv_freq_64 ? 1 : 0, amplitude, inverse ? 1 : 0, (int)first, (int)tokens, (int)T)
 #define PRL_ROPE_VEC(DT, IL) \
-  if (vec) PRL_ROPE(DT, IL, true); else PRL_ROPE(DT, IL, false)
+  if (vec && nt) PRL_ROPE(DT, IL, true, true); else if (vec) PRL_ROPE(DT, IL, true, false); else PRL_ROPE(DT, IL, false, false)
   const int64_t most = (int64_t)sh.toks << 22;  // tokens of a launch, which holds fewer than 2^32 threads
   for (int64_t first = 0; first < tokens; first += most) {
     const unsigned grid = (unsigned)(((tokens - first < most ? tokens - first : most) + sh.toks - 1) / sh.toks);

@@ -248,6 +248,11 @@ def _launch_block_norms(x: Tensor, branch: Tensor, w_post: Tensor | None, w_pre:
           None if r1 is None else r1 + 4 * rows, C.dtype_code(x), rows, h, C.stream_ptr(dev))
 
 
+@functools.lru_cache(maxsize=256)
+def _block_norms_workspace(code: int, rows: int, h: int) -> int:
+    return C.load().prl_block_norms_bwd_workspace_bytes(code, rows, h)
+
+
 class _BlockNorms(torch.autograd.Function):
     """x, branch [rows, h] and the gate in one of its three layouts; see `block_norms`."""
 
@@ -286,7 +291,7 @@ class _BlockNorms(torch.autograd.Function):
         code = C.dtype_code(x)
         ws, ws_bytes = None, 0
         if g1 is not None or g2 is not None or (gg is not None and kind in (C.GATE_CHANNEL, C.GATE_ONE)):
-            ws_bytes = lib.prl_block_norms_bwd_workspace_bytes(code, rows, h)
+            ws_bytes = _block_norms_workspace(code, rows, h)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         r1 = rstd.data_ptr()
         C.run(lib.prl_block_norms_bwd, "prl_block_norms_bwd", dev, x.data_ptr(), x.stride(0), branch.data_ptr(),
