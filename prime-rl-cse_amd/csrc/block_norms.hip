@@ -15,8 +15,10 @@
 // h, and the backward forms h again from x and b rather than reading the rounded one: the same bytes, and no gradient
 // sees that rounding.
 //
-// Bound by HBM.  A row stays in registers, EPT elements a thread, between the two sums it needs; the column sums of
-// the weight gradients stay in registers over all rows a workgroup takes and leave it once.
+// Bound by HBM: 8192 rows of 5120 bf16 with a gate per channel take 62 us forward (336 MB, 5.4 TB/s) and 103 backward
+// with its finish (503 MB, 4.9 TB/s), 16384 rows of 1024 without a gate 26 and 44 us.  A row stays in registers, four to
+// sixteen elements a thread, between the two sums it needs; the column sums of the weight gradients stay in registers
+// over all rows a workgroup takes and leave it once.
 #include <initializer_list>
 
 #include "logprob_dev.h"
@@ -24,28 +26,34 @@
 namespace prl {
 
 constexpr int kBnMaxH = 8192;
-enum { kBnElems = 0, kBnVec = 1, kBnStream = 2 };  // single elements; vectors; vectors past the caches
+constexpr int kBnStream = 2;              // non-temporal
+constexpr int kBnNoLoads = 0x0f70;        // s_waitcnt vmcnt(0), the other counters free
 constexpr int kBnRsrcFlags = 0x00020000;  // raw buffer, 32-bit data format (gfx9 family descriptor word 3)
 
-// A thread reads its share of a row in units of four registers.  In the vector modes a unit is 16 consecutive bytes, unit v at
+// A thread reads its share of a row in units of four registers.  VEC: a unit is 16 consecutive bytes, unit v at
 // 16 v, for rows whose every unit is whole and aligned.  Otherwise it is four single elements, `tpr` apart, so that a
 // wave's accesses lie side by side whatever the row's alignment: 16-byte accesses at odd places ran at half the
 // rate (8192 rows of 1531 bf16, a gate per element: forward 45.0 us against 31.8, backward 82.6 against 53.4).
+// Vector loads go past the caches and stores stay in them, for the kernel that reads them next.  Cold inputs and outputs,
+// no gate; neither past the caches, loads only, both:
+//     8192 rows of 5120 bf16, forward alone   63.7   63.0   57.3 us      its backward alone          101.2   97.0   89.8
+//     one input just written, result read      132.9  113.5  116.6                                   173.4  145.2  148.4
+//     16384 rows of 1024, the same forward     50.6   50.1   52.4        backward                     67.9   65.9   69.4
+//     2051 rows of 1536                        15.2   15.1   14.6                                     23.1   23.0   23.4
+// Single elements are read through the caches (8192 rows of 1531, a gate per element: 31.4 us against 34.0 past them).
 // Rows are read through descriptors of exactly their bytes: lanes beyond the end, and every lane of a tensor that is
 // not there, read 0 and store nothing, without a branch.
-template <int DT, int MODE>
+template <int DT, bool VEC>
 struct BnUnit {
-  static constexpr bool VEC = MODE != kBnElems;
-  static constexpr int kAux = MODE == kBnStream ? 2 : 0;  // non-temporal
   static constexpr int kEs = DT == PRL_F32 ? 4 : 2;
   static constexpr int kN = VEC ? 16 / kEs : 4;  // elements
   // column of element i of unit k of thread li
   static __device__ __forceinline__ int column(int k, int i, int li, int tpr) {
     return VEC ? (li + k * tpr) * kN + i : li + (k * kN + i) * tpr;
   }
-  template <int AUX = kAux>
-  static __device__ __forceinline__ u32x4 load(const char* row, int k, int li, int tpr, int H) {
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(row), 0, row ? H * kEs : 0, kBnRsrcFlags);
+  template <int AUX = VEC ? kBnStream : 0>
+  static __device__ __forceinline__ u32x4 load(const char* row, int bytes, int k, int li, int tpr) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(row), 0, bytes, kBnRsrcFlags);
     if constexpr (VEC) return __builtin_amdgcn_raw_buffer_load_b128(rsrc, (li + k * tpr) * 16, 0, AUX);
     uint32_t w[4];
 #pragma unroll
@@ -74,7 +82,7 @@ struct BnUnit {
       } else {
         z.x = pack_bf16(y[0], y[1]), z.y = pack_bf16(y[2], y[3]), z.z = pack_bf16(y[4], y[5]), z.w = pack_bf16(y[6], y[7]);
       }
-      __builtin_amdgcn_raw_buffer_store_b128(z, rsrc, (li + k * tpr) * 16, 0, kAux);
+      __builtin_amdgcn_raw_buffer_store_b128(z, rsrc, (li + k * tpr) * 16, 0, 0);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -128,11 +136,15 @@ __device__ __forceinline__ float bn_row_sum(float v, float* slots) {
 // Floats from one partial row to the next: whole cache lines.
 __host__ __device__ __forceinline__ int64_t bn_part_pitch(int64_t H) { return (H + 31) / 32 * 32; }
 
-struct BnRows {  // base address and row pitch in bytes
+struct BnRows {  // base address, row pitch and bytes of a row (0 for a tensor that is not there)
   const char* p;
   int64_t pitch;
-  __device__ __forceinline__ const char* row(int64_t r) const { return p ? p + r * pitch : nullptr; }
+  int bytes;
+  __device__ __forceinline__ const char* row(int64_t r) const { return p + r * pitch; }
 };
+static BnRows bn_rows(const void* p, int64_t stride, int64_t H, int64_t es) {
+  return {(const char*)p, p ? stride * es : 0, p ? (int)(H * es) : 0};
+}
 struct BnRowsOut {
   char* p;
   int64_t pitch;
@@ -165,16 +177,16 @@ struct BnIn {
   int gate_kind;
 };
 
-template <int DT, int NV, bool BWD, int GATE, int MODE>
-__device__ __forceinline__ void bn_fetch(BnRow<NV, BWD, GATE>& r, const BnIn& in, int64_t row, int li, int tpr, int H) {
-  using U = BnUnit<DT, MODE>;
+template <int DT, int NV, bool BWD, int GATE, bool VEC>
+__device__ __forceinline__ void bn_fetch(BnRow<NV, BWD, GATE>& r, const BnIn& in, int64_t row, int li, int tpr) {
+  using U = BnUnit<DT, VEC>;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    r.b[k] = U::load(in.b.row(row), k, li, tpr, H);
-    r.x[k] = U::load(in.x.row(row), k, li, tpr, H);
-    if (BWD) r.gy[k] = U::load(in.gy.row(row), k, li, tpr, H);
-    if (BWD) r.gh[k] = U::load(in.gh.row(row), k, li, tpr, H);
-    if (GATE == 2) r.g[k] = U::load(in.gate.row(row), k, li, tpr, H);
+    r.b[k] = U::load(in.b.row(row), in.b.bytes, k, li, tpr);
+    r.x[k] = U::load(in.x.row(row), in.x.bytes, k, li, tpr);
+    if (BWD) r.gy[k] = U::load(in.gy.row(row), in.gy.bytes, k, li, tpr);
+    if (BWD) r.gh[k] = U::load(in.gh.row(row), in.gh.bytes, k, li, tpr);
+    if (GATE == 2) r.g[k] = U::load(in.gate.row(row), in.gate.bytes, k, li, tpr);
   }
   r.r1 = BWD && in.rstd1 ? in.rstd1[row] : 1.0f;
   r.r2 = BWD && in.rstd2 ? in.rstd2[row] : 0.0f;
@@ -182,16 +194,16 @@ __device__ __forceinline__ void bn_fetch(BnRow<NV, BWD, GATE>& r, const BnIn& in
 }
 
 // What a thread reads once: its columns of the weights and of a gate per channel.
-template <int DT, int NV, int GATE, int MODE>
+template <int DT, int NV, int GATE, bool VEC>
 struct BnCols {
-  using U = BnUnit<DT, MODE>;
+  using U = BnUnit<DT, VEC>;
   u32x4 w1[NV], w2[NV], g[GATE ? NV : 1];
   __device__ __forceinline__ void load(const BnIn& in, int li, int tpr, int H) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      w1[k] = U::template load<0>(in.w1, k, li, tpr, H);
-      w2[k] = U::template load<0>(in.w2, k, li, tpr, H);
-      if (GATE == 1) g[k] = U::template load<0>(in.gate.p, k, li, tpr, H);
+      w1[k] = U::template load<0>(in.w1, in.w1 ? H * U::kEs : 0, k, li, tpr);
+      w2[k] = U::template load<0>(in.w2, in.w2 ? H * U::kEs : 0, k, li, tpr);
+      if (GATE == 1) g[k] = U::template load<0>(in.gate.p, H * U::kEs, k, li, tpr);
     }
   }
   // Keeps them packed through the loop over rows: the compiler would unpack what does not change in front of it, into
@@ -210,12 +222,12 @@ struct BnCols {
 
 // ONEWAVE: a wave per row, blockDim / 64 rows at a time; otherwise a workgroup per row.  The next row's loads go out
 // as soon as this one's are unpacked and stay in flight while it is worked on.  BOTH: both weights are there.
-template <int DT, int NV, bool ONEWAVE, int GATE, int MODE, bool BOTH>
+template <int DT, int NV, bool ONEWAVE, int GATE, bool VEC, bool BOTH>
 __global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_fwd(BnIn in, float scale, float offset, float eps1,
                                                                           float eps2, BnRowsOut h, BnRowsOut y,
                                                                           float* __restrict__ rstd1,
                                                                           float* __restrict__ rstd2, int64_t rows, int H) {
-  using U = BnUnit<DT, MODE>;
+  using U = BnUnit<DT, VEC>;
   constexpr int VE = U::kN;
   const bool has1 = BOTH || in.w1 != nullptr, has2 = BOTH || in.w2 != nullptr;
   __shared__ float slots[2][16];
@@ -226,10 +238,11 @@ __global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_fwd(BnIn i
   int64_t row = (int64_t)blockIdx.x * (ONEWAVE ? blockDim.x >> 6 : 1) +
                 (ONEWAVE ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
   if (row >= rows) return;
-  BnCols<DT, NV, GATE, MODE> w;
+  BnCols<DT, NV, GATE, VEC> w;
   BnRow<NV, false, GATE> cur;
-  bn_fetch<DT, NV, false, GATE, MODE>(cur, in, row, li, tpr, H);
+  bn_fetch<DT, NV, false, GATE, VEC>(cur, in, row, li, tpr);
   w.load(in, li, tpr, H);
+  __builtin_amdgcn_s_waitcnt(kBnNoLoads);  // (see k_block_norms_bwd)
   for (;;) {
     const int64_t next = row + step;
     w.keep();
@@ -247,7 +260,7 @@ __global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_fwd(BnIn i
       for (int i = 0; i < VE; ++i) ss = fmaf(bv[k][i], bv[k][i], ss);
     }
     const float gt = cur.gt;
-    if (next < rows) bn_fetch<DT, NV, false, GATE, MODE>(cur, in, next, li, tpr, H);
+    if (next < rows) bn_fetch<DT, NV, false, GATE, VEC>(cur, in, next, li, tpr);
     float r1 = 1.0f;
     if (has1) {
       r1 = rsqrtf(bn_row_sum<ONEWAVE>(ss, slots[0]) * inv_h + eps1);
@@ -297,13 +310,13 @@ __global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_fwd(BnIn i
 
 // part[array][blockIdx.x][H]: arrays 0 gw1, 1 gw2, 2 a channel gate's gradient (for a gate of one value: [blockIdx.x]),
 // each there only when asked for
-template <int DT, int NV, bool ONEWAVE, int GATE, int MODE, bool BOTH>
+template <int DT, int NV, bool ONEWAVE, int GATE, bool VEC, bool BOTH>
 __global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_bwd(BnIn in, float scale, float offset, BnRowsOut gx,
                                                                           BnRowsOut gb, float* __restrict__ part1,
                                                                           float* __restrict__ part2,
                                                                           float* __restrict__ partg, BnRowsOut gg,
                                                                           int64_t rows, int H) {
-  using U = BnUnit<DT, MODE>;
+  using U = BnUnit<DT, VEC>;
   constexpr int VE = U::kN;
   const bool has1 = BOTH || in.w1 != nullptr, has2 = BOTH || in.w2 != nullptr;
   __shared__ float slots[3][16];
@@ -320,10 +333,13 @@ __global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_bwd(BnIn i
 #pragma unroll
     for (int i = 0; i < VE; ++i) a1[k][i] = a2[k][i] = ag[GATE == 1 ? k : 0][i] = 0.0f;
   int64_t row = (int64_t)blockIdx.x * rpb + slot;
-  BnCols<DT, NV, GATE, MODE> w;
+  BnCols<DT, NV, GATE, VEC> w;
   BnRow<NV, true, GATE> cur;
-  if (row < rows) bn_fetch<DT, NV, true, GATE, MODE>(cur, in, row, li, tpr, H);
+  if (row < rows) bn_fetch<DT, NV, true, GATE, VEC>(cur, in, row, li, tpr);
   w.load(in, li, tpr, H);
+  // Nothing outstanding on entry: the loop then waits for its own loads by their number and never for the stores
+  // behind them.
+  __builtin_amdgcn_s_waitcnt(kBnNoLoads);
   while (row < rows) {
     const int64_t next = row + step;
     w.keep();
@@ -364,7 +380,7 @@ __global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_bwd(BnIn i
         }
       }
     }
-    if (next < rows) bn_fetch<DT, NV, true, GATE, MODE>(cur, in, next, li, tpr, H);
+    if (next < rows) bn_fetch<DT, NV, true, GATE, VEC>(cur, in, next, li, tpr);
     if (has2) dot = bn_row_sum<ONEWAVE>(dot, slots[0]) * inv_h;
     float dot1 = 0.0f, gdot = 0.0f;
 #pragma unroll
@@ -429,10 +445,10 @@ __global__ __launch_bounds__(ONEWAVE ? 256 : 1024) void k_block_norms_bwd(BnIn i
     for (int k = 0; k < NV; ++k) {
       const float* z = a == 0 ? a1[k] : a == 1 ? a2[k] : ag[GATE == 1 ? k : 0];
 #pragma unroll
-      for (int i = 0; i < VE; i += U::VEC ? 4 : 1) {
+      for (int i = 0; i < VE; i += VEC ? 4 : 1) {
         const int c = U::column(k, i, li, tpr);
         if (c >= H) continue;
-        if (U::VEC) *reinterpret_cast<float4*>(mine + c) = make_float4(z[i], z[i + 1], z[i + 2], z[i + 3]);
+        if (VEC) *reinterpret_cast<float4*>(mine + c) = make_float4(z[i], z[i + 1], z[i + 2], z[i + 3]);
         else mine[c] = z[i];
       }
     }
@@ -505,17 +521,16 @@ static int bn_blocks(int64_t rows, int rpb, int cap) {
   return (int)(want < cap ? (want > 0 ? want : 1) : cap);
 }
 
-// Forward: one row per wave or workgroup and as many workgroups as there are rows, except for the widest rows (7 waves
-// and more), where few workgroups that fetch the next row while they wait for this one's sums are ahead (8192 rows of
-// 5120 bf16: 65.1 us with 256 workgroups, 75 with one per row; 16384 rows of 2048: 48.5 us with one per row, 54 with
-// 1024).
+// Forward: rows of one wave each have their own; of wider rows few workgroups take many, and fetch the next row while
+// they wait for this one's sums (8192 rows of 5120 bf16: 62.1 us with 256 workgroups, 74.6 with one per row; 8192 rows of
+// 1531: 30.7 against 33.4; 16384 rows of 2048: 53.3 against 52.8).
 static int bn_fwd_blocks(int64_t rows, const BnShape& sh) {
   const int waves = sh.threads / 64;
-  return bn_blocks(rows, sh.rpb, sh.onewave || waves < 7 ? 1 << 20 : 256 * (waves < 16 ? 16 / waves : 1));
+  return bn_blocks(rows, sh.rpb, sh.onewave ? 1 << 20 : 256 * (waves < 16 ? 16 / waves : 1));
 }
 // Backward: every workgroup leaves a partial row per weight, so as few as keep 8 waves on each compute unit (16 where
-// the accesses are single elements): 8192 rows of 5120 bf16 101 us with 256, 122 with 512; 16384 rows of 2048 84 us with
-// 512, 106 with 256.
+// the accesses are single elements): 16384 rows of 2048 bf16 79.3 us with 512 workgroups, 86.4 with 1024; 8192 rows of
+// 1531 52.9 with 16 waves, 79.5 with 8.
 static int bn_bwd_blocks(int64_t rows, const BnShape& sh, bool vec) {
   const int waves = sh.threads / 64, want = vec ? 8 : 16;
   return bn_blocks(rows, sh.rpb, 256 * (want > waves ? want / waves : 1));
@@ -556,46 +571,34 @@ static int bn_check(const char* who, int dtype, int64_t rows, int64_t H, int gat
   return PRL_OK;
 }
 
-#define PRL_BN_GATE(KERNEL, DT, NV, OW, MODE, BOTH)                                     \
+#define PRL_BN_GATE(KERNEL, DT, NV, OW, VEC, BOTH)                                      \
   do {                                                                                  \
-    if (gate_kind == PRL_GATE_FULL) KERNEL(DT, NV, OW, 2, MODE, BOTH);                  \
-    else if (gate_kind == PRL_GATE_CHANNEL) KERNEL(DT, NV, OW, 1, MODE, BOTH);          \
-    else KERNEL(DT, NV, OW, 0, MODE, BOTH);                                             \
+    if (gate_kind == PRL_GATE_FULL) KERNEL(DT, NV, OW, 2, VEC, BOTH);                   \
+    else if (gate_kind == PRL_GATE_CHANNEL) KERNEL(DT, NV, OW, 1, VEC, BOTH);           \
+    else KERNEL(DT, NV, OW, 0, VEC, BOTH);                                              \
   } while (0)
-// (the streaming form only with both weights)
-#define PRL_BN_MODE(KERNEL, DT, NV, OW)                                            \
-  do {                                                                             \
-    const bool both = w_post && w_pre;                                             \
-    if (vec && both && stream_past) PRL_BN_GATE(KERNEL, DT, NV, OW, kBnStream, true); \
-    else if (vec && both) PRL_BN_GATE(KERNEL, DT, NV, OW, kBnVec, true);           \
-    else if (vec) PRL_BN_GATE(KERNEL, DT, NV, OW, kBnVec, false);                  \
-    else if (both) PRL_BN_GATE(KERNEL, DT, NV, OW, kBnElems, true);                \
-    else PRL_BN_GATE(KERNEL, DT, NV, OW, kBnElems, false);                         \
+#define PRL_BN_VEC(KERNEL, DT, NV, OW, VEC)                            \
+  do {                                                                 \
+    if (w_post && w_pre) PRL_BN_GATE(KERNEL, DT, NV, OW, VEC, true);   \
+    else PRL_BN_GATE(KERNEL, DT, NV, OW, VEC, false);                  \
   } while (0)
-#define PRL_BN_ELEMS(KERNEL, DT, NV, OW)                                     \
-  do {                                                                       \
-    if (w_post && w_pre) PRL_BN_GATE(KERNEL, DT, NV, OW, kBnElems, true);    \
-    else PRL_BN_GATE(KERNEL, DT, NV, OW, kBnElems, false);                   \
+#define PRL_BN_SHAPE(KERNEL, DT, VEC)                                   \
+  do {                                                                  \
+    if (sh.onewave && sh.nv == 1) PRL_BN_VEC(KERNEL, DT, 1, true, VEC); \
+    else if (sh.onewave) PRL_BN_VEC(KERNEL, DT, 2, true, VEC);          \
+    else PRL_BN_VEC(KERNEL, DT, 1, false, VEC);                         \
   } while (0)
 #define PRL_BN_DISPATCH(KERNEL)                                                           \
   do { /* (two units a thread of a workgroup: rows of more than 4096 fp32 or single elements) */ \
     const bool wide = !sh.onewave && sh.nv == 2;                                          \
-    if (dtype == PRL_F32) {                                                               \
-      if (wide) PRL_BN_MODE(KERNEL, PRL_F32, 2, false);                                   \
-      else if (!sh.onewave) PRL_BN_MODE(KERNEL, PRL_F32, 1, false);                       \
-      else if (sh.nv == 1) PRL_BN_MODE(KERNEL, PRL_F32, 1, true);                         \
-      else PRL_BN_MODE(KERNEL, PRL_F32, 2, true);                                         \
-    } else {                                                                              \
-      if (wide) PRL_BN_ELEMS(KERNEL, PRL_BF16, 2, false);                                 \
-      else if (!sh.onewave) PRL_BN_MODE(KERNEL, PRL_BF16, 1, false);                      \
-      else if (sh.nv == 1) PRL_BN_MODE(KERNEL, PRL_BF16, 1, true);                        \
-      else PRL_BN_MODE(KERNEL, PRL_BF16, 2, true);                                        \
-    }                                                                                     \
+    if (dtype == PRL_F32 && vec && wide) PRL_BN_VEC(KERNEL, PRL_F32, 2, false, true);     \
+    else if (dtype == PRL_F32 && vec) PRL_BN_SHAPE(KERNEL, PRL_F32, true);                \
+    else if (dtype == PRL_F32 && wide) PRL_BN_VEC(KERNEL, PRL_F32, 2, false, false);      \
+    else if (dtype == PRL_F32) PRL_BN_SHAPE(KERNEL, PRL_F32, false);                      \
+    else if (vec) PRL_BN_SHAPE(KERNEL, PRL_BF16, true);                                   \
+    else if (wide) PRL_BN_VEC(KERNEL, PRL_BF16, 2, false, false);                         \
+    else PRL_BN_SHAPE(KERNEL, PRL_BF16, false);                                           \
   } while (0)
-
-// Past the caches from 64 MB on, which would not stay there for the next kernel either (8192 rows of 5120 bf16, forward 64
-// -> 60 us, backward 100 -> 95).
-static bool bn_stream_past(int64_t tensors, int64_t rows, int64_t H, int64_t es) { return tensors * rows * H * es >= (64 << 20); }
 
 extern "C" int prl_block_norms_fwd(const void* x, int64_t x_stride, const void* branch, int64_t branch_stride,
                                    const void* w_post, const void* w_pre, int gate_kind, const void* gate,
@@ -619,11 +622,11 @@ extern "C" int prl_block_norms_fwd(const void* x, int64_t x_stride, const void* 
                               gate_kind == PRL_GATE_FULL ? gate_stride : 0});
   const BnShape sh = bn_shape(dtype, H, vec);
   const dim3 grid((unsigned)bn_fwd_blocks(rows, sh)), block((unsigned)sh.threads);
-  const BnIn in = {{(const char*)x, x_stride * es}, {(const char*)branch, branch_stride * es}, {nullptr, 0}, {nullptr, 0},
-                   {(const char*)gate, gate_pitch}, nullptr, nullptr, (const char*)w_post, (const char*)w_pre, gate_kind};
-  const bool stream_past = bn_stream_past(4, rows, H, es);
-#define PRL_BN_FWD(DT, NV, OW, GATE, MODE, BOTH)                                                                       \
-  hipLaunchKernelGGL((k_block_norms_fwd<DT, NV, OW, GATE, MODE, BOTH>), grid, block, 0, (hipStream_t)stream, in, scale, \
+  const BnIn in = {bn_rows(x, x_stride, H, es), bn_rows(branch, branch_stride, H, es), {}, {},
+                   {(const char*)gate, gate_pitch, (int)(H * es)}, nullptr, nullptr, (const char*)w_post,
+                   (const char*)w_pre, gate_kind};
+#define PRL_BN_FWD(DT, NV, OW, GATE, VEC, BOTH)                                                                       \
+  hipLaunchKernelGGL((k_block_norms_fwd<DT, NV, OW, GATE, VEC, BOTH>), grid, block, 0, (hipStream_t)stream, in, scale, \
                      weight_offset, eps_post, eps_pre, (BnRowsOut{(char*)hidden, hidden_stride * es}),                \
                      (BnRowsOut{(char*)normed, n_stride * es}), w_post ? rstd_post : nullptr,                         \
                      w_pre ? rstd_pre : nullptr, rows, (int)H)
@@ -677,19 +680,18 @@ extern "C" int prl_block_norms_bwd(const void* x, int64_t x_stride, const void* 
   const dim3 grid((unsigned)nblk), block((unsigned)sh.threads);
   const size_t lds = sh.onewave ? (size_t)sh.rpb * bn_part_pitch(H) * sizeof(float) : 0;
   char* gg = channel || !g_gate ? nullptr : (char*)g_gate;
-  const BnIn in = {{(const char*)x, x_stride * es},
-                   {(const char*)branch, branch_stride * es},
-                   {(const char*)g_normed, g_normed_stride * es},
-                   {(const char*)g_hidden, g_hidden_stride * es},
-                   {(const char*)gate, gate_pitch},
+  const BnIn in = {bn_rows(x, x_stride, H, es),
+                   bn_rows(branch, branch_stride, H, es),
+                   bn_rows(g_normed, g_normed_stride, H, es),
+                   bn_rows(g_hidden, g_hidden_stride, H, es),
+                   {(const char*)gate, gate_pitch, (int)(H * es)},
                    w_post ? rstd_post : nullptr,
                    w_pre ? rstd_pre : nullptr,
                    (const char*)w_post,
                    (const char*)w_pre,
                    gate_kind};
-  const bool stream_past = bn_stream_past(6, rows, H, es);
-#define PRL_BN_BWD(DT, NV, OW, GATE, MODE, BOTH)                                                                       \
-  hipLaunchKernelGGL((k_block_norms_bwd<DT, NV, OW, GATE, MODE, BOTH>), grid, block, lds, st, in, scale, weight_offset, \
+#define PRL_BN_BWD(DT, NV, OW, GATE, VEC, BOTH)                                                                       \
+  hipLaunchKernelGGL((k_block_norms_bwd<DT, NV, OW, GATE, VEC, BOTH>), grid, block, lds, st, in, scale, weight_offset, \
                      (BnRowsOut{(char*)gx, gx_stride * es}), (BnRowsOut{(char*)g_branch, g_branch_stride * es}), p1, p2, \
                      pg, (BnRowsOut{gg, g_gate_stride * es}), rows, (int)H)
   PRL_BN_DISPATCH(PRL_BN_BWD);

@@ -11,9 +11,9 @@
 // It is formed in fp64 in turns, p f / (2 pi), and only its fraction of a turn goes to fp32, where sincospi is good to
 // fp32 rounding.
 //
-// Bound by HBM: every element read and written once.  A workgroup takes a few tokens and forms their cos / sin once in
-// LDS (r / 2 pairs per token).  A thread then owns one place in the head, two 16-byte vectors of it, keeps its cos / sin
-// in registers and walks over the heads of query and key, two at a time: no index arithmetic between heads.
+// Bound by HBM: every element read and written once, 201 MB in 39.5 us (5.1 TB/s).  A workgroup takes a few tokens and
+// forms their cos / sin once in LDS (r / 2 pairs per token).  A thread then owns one place in the head, two 16-byte
+// vectors of it, keeps its cos / sin in registers and walks over the heads of query and key, two at a time.
 #include "logprob_dev.h"
 
 namespace prl {
@@ -38,8 +38,8 @@ struct RopeSide {
 };
 
 // VEC: a thread's two pieces of a head are 16-byte vectors (rows aligned, the pairs of the half layout in whole vectors);
-// otherwise single elements, side by side over the lanes (r = 34 of 128 in the half layout:
-// 53.5 us; 16-byte accesses at places aligned to an element only took 107).
+// otherwise single elements, side by side over the lanes (r = 34 of 128 in the half layout: 49.2 us; 16-byte accesses at
+// places aligned to an element only took 107).  NT: the loads go past the caches.
 template <int DT, bool VEC, bool NT>
 struct RopeUnit {
   static constexpr int kEs = DT == PRL_F32 ? 4 : 2;
@@ -56,8 +56,7 @@ struct RopeUnit {
     else y[0] = DT == PRL_F32 ? __uint_as_float(z.x) : bf16_lo(z.x);
   }
   __device__ __forceinline__ void store(char* p) const {
-    if constexpr (VEC && NT) __builtin_nontemporal_store(z, reinterpret_cast<u32x4*>(p));
-    else if constexpr (VEC) *reinterpret_cast<u32x4*>(p) = z;
+    if constexpr (VEC) *reinterpret_cast<u32x4*>(p) = z;
     else if constexpr (DT == PRL_F32) *reinterpret_cast<uint32_t*>(p) = z.x;
     else *reinterpret_cast<uint16_t*>(p) = (uint16_t)z.x;
   }
@@ -180,8 +179,8 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope_positions(RopeSide q, Rop
 }
 
 // Threads of a workgroup: `units` side by side on a row as far as they go, the rest over two tokens and as many heads of
-// each as fit (16384 tokens of 24 heads of 128 bf16, 201 MB: 41.1 us with two tokens, 49.0 with one, 42.3 with four;
-// 48 single tokens: 4.2 us with one, two or four).
+// each as fit (24 heads of 128 bf16, 16384 tokens: 39.5 us with two tokens, 50.5 with one, 39.7 with four; 2048 tokens:
+// 7.2, 8.4, 8.3; 48 single tokens: 4.2 with any).
 static RopeShape rope_shape(int64_t r, int64_t D, int64_t heads, int ve, bool il, bool vec) {
   RopeShape s;
   s.r = (int)r, s.D = (int)D;
@@ -242,10 +241,11 @@ extern "C" int prl_rope_positions(const void* q, void* q_out, const int64_t* q_s
   // every 16-byte access of a row starts a multiple of 16 bytes from the row's start
   const bool vec = ((bits | (uintptr_t)(D * es) | (uintptr_t)(interleaved ? 0 : half * es)) & 15) == 0;
   const int64_t tokens = B * T;
-  // Past the caches where what is moved would not stay there and a wave's accesses are whole lines (201 MB: 36.6 us
-  // against 41.0; 25 MB: 6.9 against 6.7; 201 MB with 32 of 128 dimensions turned in halves, where a row's pieces lie
-  // scattered: 43.6 against 40.3).
-  const bool nt = 2 * tokens * heads * D * es >= (64 << 20) && (interleaved || rotary_dim == D);
+  // Loads go past the caches where a wave's accesses are whole lines (half of 128 dimensions turned in halves, 167 MB:
+  // 83.8 us against 81.0 through them), stores stay in them for the attention that reads them.  Cold, one side just
+  // written and read behind; neither past the caches, loads only, both: 25 MB 20.8, 20.4, 20.8 us; 167 MB 81.2, 80.3,
+  // 82.4; 402 MB 213, 208, 202; by itself 402 MB 75.3, 74.7, 69.0.
+  const bool nt = interleaved || rotary_dim == D;
   const RopeShape sh = rope_shape(rotary_dim, D, heads, ve, interleaved, vec);
   const size_t lds = (size_t)sh.toks * half * sizeof(float2);
 #define PRL_ROPE(DT, IL, VEC, NT)                                                                                       \
