@@ -432,12 +432,20 @@ def apply_rotary_pos_emb(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, unsquee
 
 
 class _RopeSource:
-    """Where a rotary module's cos / sin came from: what `rope_at_positions` takes instead of them."""
+    """Where a rotary module's cos / sin came from: what `rope_at_positions` takes instead of them, as long as none of
+    these tensors was written since (`stands`)."""
 
-    __slots__ = ("position_ids", "inv_freq", "amplitude")
+    __slots__ = ("position_ids", "inv_freq", "amplitude", "sin", "versions")
 
-    def __init__(self, position_ids: Tensor, inv_freq: Tensor, amplitude: float):
-        self.position_ids, self.inv_freq, self.amplitude = position_ids, inv_freq, amplitude
+    def __init__(self, position_ids: Tensor, inv_freq: Tensor, amplitude: float, cos: Tensor, sin: Tensor):
+        self.position_ids, self.inv_freq, self.amplitude, self.sin = position_ids, inv_freq, amplitude, sin
+        self.versions = self._count(cos)
+
+    def _count(self, cos: Tensor) -> tuple[int, ...]:
+        return cos._version, self.sin._version, self.position_ids._version, self.inv_freq._version
+
+    def stands(self, cos: Tensor, sin: Tensor) -> bool:
+        return sin is self.sin and self._count(cos) == self.versions
 
 
 def _tagged_rotary_forward(self: nn.Module, x: Tensor, position_ids: Tensor, *args: Any, **kwargs: Any):
@@ -449,7 +457,8 @@ def _tagged_rotary_forward(self: nn.Module, x: Tensor, position_ids: Tensor, *ar
     inv_freq = self.inv_freq  # (read after the call: frequencies that depend on the length are set in there)
     if inv_freq.dtype != torch.float32:
         inv_freq = inv_freq.float()  # as the module itself uses it
-    cos._prl_rope = _RopeSource(position_ids, inv_freq, float(getattr(self, "attention_scaling", 1.0)))
+    if not any(t.is_inference() for t in (cos, sin, position_ids, inv_freq)):  # (those count no writes)
+        cos._prl_rope = _RopeSource(position_ids, inv_freq, float(getattr(self, "attention_scaling", 1.0)), cos, sin)
     return cos, sin
 
 
@@ -461,7 +470,7 @@ def _family_rope(original: Any, kind: str) -> Any:
     def rotate(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, *args: Any, **kwargs: Any):
         if not args and not kwargs or (kwargs == {"unsqueeze_dim": 1} and not args) or (args == (1,) and not kwargs):
             source = getattr(cos, "_prl_rope", None)
-            if source is None:
+            if source is None or not source.stands(cos, sin):
                 if kind == "half" and rope_supported(q, k, cos, sin):
                     return _Rope.apply(q, k, cos, sin)
             elif rope_at_positions_supported(q, k, source.position_ids, source.inv_freq):
@@ -1128,26 +1137,27 @@ _NORM_FORMS: dict[type, float | None] = {}
 def _norm_form(norm: nn.Module) -> float | None:
     """What is added to a normalisation module's weight (0 or 1) if it is an RMSNorm of the last dimension, found by
     what its forward does to a small host tensor; None otherwise."""
+    weight, eps = getattr(norm, "weight", None), _norm_eps(norm)
+    if not isinstance(weight, Tensor) or weight.ndim != 1 or eps is None or list(norm.children()):
+        return None
     cls = type(norm)
     if cls not in _NORM_FORMS:
         import copy
 
         _NORM_FORMS[cls] = None
-        weight, eps = getattr(norm, "weight", None), _norm_eps(norm)
-        if isinstance(weight, Tensor) and weight.ndim == 1 and eps is not None and not list(norm.children()):
-            gen = torch.Generator().manual_seed(0)
-            x, w = torch.randn(3, 8, generator=gen), torch.randn(8, generator=gen)
-            try:
-                probe = copy.copy(norm)
-                probe._parameters = {"weight": nn.Parameter(w, requires_grad=False)}
-                with torch.no_grad():
-                    got = cls.forward(probe, x)
-                unit = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + eps)
-                for offset in (0.0, 1.0):
-                    if torch.allclose(got, unit * (w + offset), rtol=1e-5, atol=1e-6):
-                        _NORM_FORMS[cls] = offset
-            except Exception:
-                pass
+        gen = torch.Generator().manual_seed(0)
+        x, w = torch.randn(3, 8, generator=gen), torch.randn(8, generator=gen)
+        try:
+            probe = copy.copy(norm)
+            probe._parameters = {"weight": nn.Parameter(w, requires_grad=False)}
+            with torch.no_grad():
+                got = cls.forward(probe, x)
+            unit = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + eps)
+            for offset in (0.0, 1.0):
+                if torch.allclose(got, unit * (w + offset), rtol=1e-5, atol=1e-6):
+                    _NORM_FORMS[cls] = offset
+        except Exception:
+            pass
     return _NORM_FORMS[cls]
 
 

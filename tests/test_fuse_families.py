@@ -80,3 +80,43 @@ def test_form_of_the_norms():
     assert fused._norm_form(tiny("Gemma2").model.norm) == 1.0
     assert fused._norm_form(torch.nn.LayerNorm(8)) is None
     assert fused._norm_form(tiny("Cohere").model.norm) is None
+
+
+@pytest.mark.parametrize("change", [None, "cos", "sin", "positions", "other"])
+def test_tables_that_were_changed_are_not_replaced_by_positions(change, monkeypatch):
+    """The positions left on a rotary module's cos stand for its tables only as long as these are what it returned."""
+    taken = []
+    monkeypatch.setattr(fused, "rope_at_positions_supported", lambda *a: True)
+    monkeypatch.setattr(fused, "rope_at_positions", lambda q, k, *a, **kw: taken.append("positions") or (q, k))
+    rotate = fused._family_rope(lambda q, k, cos, sin: taken.append("tables") or (q, k), "interleaved")
+    rotary = tiny("Glm4").model.rotary_emb
+    rotary._prl_torch_forward = rotary.forward
+    q, k, pos = torch.randn(1, 2, 5, 16), torch.randn(1, 1, 5, 16), torch.arange(5)[None]
+    cos, sin = fused._tagged_rotary_forward(rotary, q, pos)
+    if change == "other":
+        sin = sin.clone()
+    elif change:
+        {"cos": cos, "sin": sin, "positions": pos}[change].mul_(2)
+    rotate(q, k, cos, sin)
+    assert taken == ["tables" if change else "positions"]
+    taken.clear()
+    with torch.inference_mode():  # (tensors that count no writes)
+        rotate(q, k, *fused._tagged_rotary_forward(rotary, q, pos))
+    assert taken == ["tables"]
+
+
+def test_form_of_a_norm_is_asked_of_the_module_itself():
+    """A class may leave its weight out of some of its instances."""
+    class Norm(torch.nn.Module):
+        def __init__(self, scaled):
+            super().__init__()
+            self.eps = 1e-6
+            self.weight = torch.nn.Parameter(torch.ones(8)) if scaled else None
+
+        def forward(self, x):
+            y = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + self.eps)
+            return y if self.weight is None else y * self.weight
+
+    assert fused._norm_form(Norm(True)) == 0.0
+    assert fused._norm_form(Norm(False)) is None
+    assert fused._norm_form(Norm(True)) == 0.0
