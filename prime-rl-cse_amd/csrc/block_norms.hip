@@ -156,13 +156,6 @@ __device__ __forceinline__ float bn_elem(const char* p) {
   return DT == PRL_F32 ? *reinterpret_cast<const float*>(p) : bf16_one(*reinterpret_cast<const uint16_t*>(p));
 }
 
-// Places beyond a row's end read as 0 and add 0 to every sum: they are not masked.  (Only a factor that is not finite
-// makes them something else, and then the row's own values are not numbers either.)
-
-// Keeps a unit in its packed form through a loop: the compiler would unpack what does not change in front of it,
-// into twice the registers.
-__device__ __forceinline__ void bn_keep_packed(u32x4& v) { asm volatile("" : "+v"(v)); }
-
 // How the gate comes: not at all, as one value or one per row (GATE 0), one per channel (1, kept over the rows), one
 // per element (2).
 template <int NV, bool BWD, int GATE>
