@@ -8,8 +8,11 @@ model's normalisation modules to `rms_norm` (one HIP launch forward and two
 backward instead of ~22 small torch kernels) and the model family's
 `apply_rotary_pos_emb` to one launch for query and key together (instead of
 ~14 forward and ~20 backward), and the gated MLPs' `silu(gate) * up` to one
-launch each way (instead of 2 and 5).  Modules whose shape or dtype the
-kernels do not cover keep their torch forward (on the same device; nothing
+launch each way (instead of 2 and 5).  Families that turn part of a head or
+neighbouring dimensions rotate from position ids (`rope_at_positions`), and
+layers with a norm behind a block or a factor on the residual do what lies
+between two blocks in one launch (`block_norms`).  Modules whose shape or dtype
+the kernels do not cover keep their torch forward (on the same device; nothing
 moves to the host).
 """
 

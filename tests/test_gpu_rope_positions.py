@@ -146,6 +146,29 @@ def test_one_side_only_and_empty_inputs():
         assert a.shape == shape and b.shape == shape
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("r", [32, 20])
+def test_gradient_against_differences(r, interleaved):
+    """The rotation is linear: the change of a weighted sum of its outputs along v is what its gradient says times v, for
+    steps of any size.  Both sides are sums of terms whose values the kernel rounds as `check` counts."""
+    q, k = inputs(2, 11, 3, 2, 32, torch.float32, "bthd", seed=5)
+    v, _ = inputs(2, 11, 3, 2, 32, torch.float32, "bhtd", seed=6)
+    g, _ = inputs(2, 11, 3, 2, 32, torch.float32, "bhtd", seed=7)
+    inv_freq, _ = fused.rope_frequencies(r, device=DEV)
+    pos = torch.arange(11, device=DEV) * 7
+    f = lambda x: fused.rope_at_positions(x, k, pos, inv_freq, interleaved=interleaved, attention_scaling=1.25)[0]
+    leaf = q.clone().requires_grad_(True)
+    (dq,) = torch.autograd.grad(f(leaf), leaf, g)
+    up, down = q + v, q - v
+    step = (up.double() - down.double()) / 2  # what the rounded sums differ by
+    change = ((f(up).double() - f(down).double()) / 2 * g.double()).sum()
+    theta = torch.zeros((), device=DEV, dtype=torch.float64)
+    size = lambda x: turned(x, theta, 1.25, r, interleaved)[1] * 1.25 + x.double().abs()
+    part = 3.15 * 2.0**-25 + 2 * 2.0**-23 + 5 * 2.0**-24
+    tol = part * ((size(up) + size(down)) / 2 * g.double().abs()).sum() + part * (size(g) * step.abs()).sum()
+    assert abs(float(change - (dq.double() * step).sum())) <= float(tol)
+
+
 def test_a_second_derivative_is_refused():
     q, k = inputs(1, 4, 1, 1, 8, torch.float32, "bhtd")
     q.requires_grad_(True)
