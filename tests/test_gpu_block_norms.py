@@ -302,3 +302,19 @@ def test_library_leaves_what_lies_between_rows():
         C.stream_ptr(out.device)), "prl_block_norms_fwd")
     hid, y = fused.block_norms(t["x"], t["b"], t["w1"], t["w2"], eps=E1, pre_eps=E2)
     assert torch.equal(out[0, :, :h], hid) and torch.equal(out[1, :, :h], y) and bool((out[..., h:] == 7).all())
+
+
+@pytest.mark.parametrize("rows, h", [((1 << 20) + 33, 2056), ((1 << 22) + 9, 8)])  # 2.2e9 elements; more rows than waves
+def test_many_rows(rows, h):
+    """Far rows come out as they do by themselves, bit for bit, both ways."""
+    mk = lambda: torch.empty(rows, h, dtype=torch.bfloat16, device=DEV).normal_()
+    x, b, gh, gy = mk().requires_grad_(True), mk().requires_grad_(True), mk(), mk()
+    w = torch.rand(h, device=DEV).to(torch.bfloat16)
+    run = lambda x, b: fused.block_norms(x, b, w, w, scale=0.5, eps=E1, pre_eps=E2)
+    out = run(x, b)
+    grads = torch.autograd.grad(out, [x, b], [gh, gy])
+    for cut in (slice(0, 7), slice(rows // 2, rows // 2 + 7), slice(rows - 7, rows)):
+        xs, bs = (v.detach()[cut].clone().requires_grad_(True) for v in (x, b))
+        alone = run(xs, bs)
+        for got, want in zip((*out, *grads), (*alone, *torch.autograd.grad(alone, [xs, bs], [gh[cut], gy[cut]]))):
+            assert torch.equal(got[cut], want)

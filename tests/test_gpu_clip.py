@@ -196,3 +196,18 @@ def test_one_call_and_its_two_halves_agree(which):
     n1 = optim.clip_grad_norm_(a, 0.5)
     n2 = optim.clip_grad_norm_(b, 0.5, error_if_nonfinite=True)
     assert torch.equal(n1, n2) and all(torch.equal(p.grad, q.grad) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("norm_type", [2.0, math.inf])
+def test_one_gradient_of_more_than_2_31_elements(norm_type):
+    n = 2**31 + 8195
+    p = torch.empty(n, dtype=BF, device=DEV, requires_grad=True)
+    p.grad = torch.full((n,), 0.5, dtype=BF, device=DEV)
+    p.grad[-1] = -2.0  # the last element alone is the largest
+    want = math.sqrt((n - 1) * 0.25 + 4.0) if norm_type == 2.0 else 2.0
+    got = optim.clip_grad_norm_(p, want / 2, norm_type)
+    assert abs(float(got) - want) <= 2.0**-24 * (1 + 1e-6) * want
+    # halves but for 1e-6 and a few fp32 roundings, which bf16's step of 2^-8 hides
+    for cut in (slice(0, 9000), slice(2**31 - 9000, 2**31 + 8194)):
+        assert bool((p.grad[cut] == 0.25).all())
+    assert float(p.grad[-1]) == -1.0

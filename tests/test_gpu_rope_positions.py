@@ -255,3 +255,16 @@ def test_more_tokens_than_a_launch_has_workgroups_for():
     out, _ = fused.rope_at_positions(x, None, pos, f)
     for cut in (slice(0, 1000), slice((1 << 23) - 1000, n)):
         check(out[:, :, cut], x[:, :, cut], pos[cut].double()[None, None, :, None], 1.0, 2, False)
+
+
+def test_offsets_beyond_32_bits():
+    t, heads, d = (1 << 17) + 3, 130, 128  # 2.2e9 elements
+    x = torch.empty(1, t, heads, d, dtype=torch.bfloat16, device=DEV).normal_().transpose(1, 2)
+    pos = torch.arange(t, device=DEV)
+    inv_freq, _ = fused.rope_frequencies(d, device=DEV)
+    out, _ = fused.rope_at_positions(x, None, pos, inv_freq)
+    assert x.numel() > 2**31
+    for cut in (slice(0, 5), slice(t // 2, t // 2 + 5), slice(t - 5, t)):
+        alone, _ = fused.rope_at_positions(x[:, :, cut], None, pos[cut], inv_freq)
+        assert torch.equal(out[:, :, cut], alone)
+        check(alone, x[:, :, cut], pos[cut].double()[None, None, :, None] * inv_freq.double(), 1.0, d, False)
