@@ -1134,34 +1134,43 @@ def _layer_steps(module: nn.Module) -> _LayerSteps | None:
     return steps
 
 
-_NORM_FORMS: dict[type, float | None] = {}
+_UNASKED = object()
 
 
 def _norm_form(norm: nn.Module) -> float | None:
     """What is added to a normalisation module's weight (0 or 1) if it is an RMSNorm of the last dimension, found by
-    what its forward does to a small host tensor; None otherwise."""
-    weight, eps = getattr(norm, "weight", None), _norm_eps(norm)
+    what its forward does to a small host tensor; None otherwise.  Asked of every module by itself (a forward may go by
+    any attribute of the instance), once, and kept on it until the next `fuse_model`."""
+    form = norm.__dict__.get("_prl_norm_form", _UNASKED)
+    if form is _UNASKED:
+        form = norm._prl_norm_form = _probe_norm(norm)
+    return form
+
+
+def _probe_norm(norm: nn.Module) -> float | None:
+    import copy
+
+    weight, eps, cls = getattr(norm, "weight", None), _norm_eps(norm), type(norm)
     if not isinstance(weight, Tensor) or weight.ndim != 1 or eps is None or list(norm.children()):
         return None
-    cls = type(norm)
-    if cls not in _NORM_FORMS:
-        import copy
-
-        _NORM_FORMS[cls] = None
-        gen = torch.Generator().manual_seed(0)
-        x, w = torch.randn(3, 8, generator=gen), torch.randn(8, generator=gen)
-        try:
-            probe = copy.copy(norm)
-            probe._parameters = {"weight": nn.Parameter(w, requires_grad=False)}
-            with torch.no_grad():
-                got = cls.forward(probe, x)
-            unit = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + eps)
-            for offset in (0.0, 1.0):
-                if torch.allclose(got, unit * (w + offset), rtol=1e-5, atol=1e-6):
-                    _NORM_FORMS[cls] = offset
-        except Exception:
-            pass
-    return _NORM_FORMS[cls]
+    own = norm.__dict__.get("_prl_torch_forward", norm.forward)  # (what this package has bound in front of it aside)
+    if getattr(own, "__func__", None) is not cls.forward:
+        return None
+    gen = torch.Generator().manual_seed(0)
+    x, w = (torch.randn(n, 8, generator=gen, dtype=torch.float32, device="cpu") for n in (3, 1))
+    x, w = x * torch.tensor([[1.0], [1e-3], [30.0]], dtype=torch.float32, device="cpu"), w[0]  # (eps shows in the second)
+    try:
+        probe = copy.copy(norm)
+        probe._parameters = {"weight": nn.Parameter(w, requires_grad=False)}
+        with torch.no_grad():
+            got = cls.forward(probe, x)
+        unit = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + eps)
+        for offset in (0.0, 1.0):
+            if torch.allclose(got, unit * (w + offset), rtol=1e-5, atol=1e-6):
+                return offset
+    except Exception:
+        pass
+    return None
 
 
 def _norm_eps(norm: nn.Module) -> float | None:
@@ -1467,6 +1476,8 @@ def fuse_model(model: nn.Module) -> dict[str, int]:
     layers_too = os.environ.get("PRL_FUSED_LAYER", "1") != "0"  # the residual additions inside the norm kernels
 
     home = sys.modules.get(type(model).__module__)  # e.g. transformers.models.qwen3.modeling_qwen3
+    for module in model.modules():
+        module.__dict__.pop("_prl_norm_form", None)
     kind = None
     if home is not None and hasattr(home, "apply_rotary_pos_emb"):
         if home.__name__ in _PATCHED_MODULES:  # (what the patch replaced is what tells the pairs)
@@ -1557,6 +1568,7 @@ def unfuse_model(model: nn.Module) -> None:
     if home is not None and home.__name__ in _PATCHED_MODULES:
         home.apply_rotary_pos_emb = _PATCHED_MODULES.pop(home.__name__)
     for module in model.modules():
+        module.__dict__.pop("_prl_norm_form", None)
         if hasattr(module, "_prl_torch_forward"):
             module.forward = module._prl_torch_forward
             del module._prl_torch_forward

@@ -1,0 +1,62 @@
+"""Calls at the edges of the fused layers' host side: norms whose instances differ, tables, hooks, gradients that share
+memory.  Host only; the kernels' side is tests/test_gpu_operator_edges.py."""
+
+import copy
+
+import pytest
+import torch
+
+import prime_rl_cse_amd as prl  # noqa: F401
+from prime_rl_cse_amd import fused
+
+
+class FlaggedNorm(torch.nn.Module):
+    """An RMSNorm whose instances say for themselves whether the weight is a distance from one."""
+
+    def __init__(self, from_one, width=8):
+        super().__init__()
+        self.eps, self.from_one = 1e-6, from_one
+        self.weight = torch.nn.Parameter(torch.rand(width))
+
+    def forward(self, x):
+        y = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + self.eps)
+        return y * (1.0 + self.weight if self.from_one else self.weight)
+
+
+@pytest.mark.parametrize("order", [(False, True), (True, False)])
+def test_a_norm_s_form_belongs_to_the_instance(order):
+    norms = [FlaggedNorm(flag) for flag in order]
+    for _ in range(2):  # (asked again: what was found is kept on the module)
+        assert [fused._norm_form(n) for n in norms] == [float(flag) for flag in order]
+
+
+def test_a_norm_whose_forward_was_replaced_has_no_form():
+    norm = FlaggedNorm(False)
+    norm.forward = lambda x: x * 2
+    assert fused._norm_form(norm) is None
+
+
+def test_a_norm_that_uses_another_epsilon_has_no_form():
+    class Norm(FlaggedNorm):
+        def forward(self, x):
+            return x * torch.rsqrt((x * x).mean(-1, keepdim=True) + 1.5e-6) * self.weight
+
+    assert fused._norm_form(Norm(False)) is None
+
+
+def test_a_norm_s_form_is_found_under_other_defaults():
+    before = torch.get_default_dtype()
+    try:
+        torch.set_default_dtype(torch.bfloat16)
+        assert fused._norm_form(FlaggedNorm(True)) == 1.0
+    finally:
+        torch.set_default_dtype(before)
+
+
+def test_fuse_model_asks_norms_anew():
+    norm = FlaggedNorm(False)
+    assert fused._norm_form(norm) == 0.0
+    other = copy.deepcopy(norm)
+    other.from_one = True
+    fused.fuse_model(torch.nn.ModuleList([other]))
+    assert fused._norm_form(other) == 1.0 and fused._norm_form(norm) == 0.0
