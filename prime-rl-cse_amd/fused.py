@@ -1186,7 +1186,7 @@ def _between_blocks(x: Tensor, branch: Tensor, post: nn.Module | None, scale: fl
     """(x + scale post(branch), pre of it): one launch where `block_norms` takes the tensors, else step by step."""
     w1, w2 = (None if n is None else n.weight for n in (post, pre))
     forms = {_norm_form(n) for n in (post, pre) if n is not None}
-    if len(forms) <= 1 and not any(hasattr(w, "to_local") for w in (w1, w2)) \
+    if len(forms) <= 1 and None not in forms and not any(hasattr(w, "to_local") for w in (w1, w2)) \
             and block_norms_supported(x, branch, w1, w2):
         e1 = _norm_eps(post) if post is not None else 0.0
         hidden, normed = block_norms(x, branch, w1, w2, scale=scale, eps=e1, pre_eps=_norm_eps(pre) if pre is not None else e1,

@@ -60,3 +60,14 @@ def test_fuse_model_asks_norms_anew():
     other.from_one = True
     fused.fuse_model(torch.nn.ModuleList([other]))
     assert fused._norm_form(other) == 1.0 and fused._norm_form(norm) == 0.0
+
+
+@pytest.mark.parametrize("post", [False, True])
+def test_a_norm_of_unknown_form_is_called(post, monkeypatch):
+    """One norm alone, and it is none the kernel knows: step by step."""
+    monkeypatch.setattr(fused, "block_norms_supported", lambda *a, **k: True)
+    norm = torch.nn.LayerNorm(8)
+    x, branch = torch.randn(3, 8), torch.randn(3, 8)
+    hidden, normed = fused._between_blocks(x, branch, norm if post else None, 0.5, None if post else norm)
+    want = x + 0.5 * (norm(branch) if post else branch)
+    assert torch.equal(hidden, want) and torch.equal(normed, want if post else norm(want))
