@@ -958,8 +958,9 @@ class _Carry:
     def put(self, hidden: Tensor, branch: Tensor, behind: tuple[nn.Module | None, float] | None = None) -> None:
         self.hidden, self.branch, self.behind = hidden, branch, behind
 
-    def join(self, hidden: Tensor, norm: nn.Module | None) -> tuple[Tensor, Tensor] | None:
-        """(hidden with the pending branch added, `norm` of it), or None if nothing is pending."""
+    def join(self, hidden: Tensor, norm: nn.Module | None, inside: bool = False) -> tuple[Tensor, Tensor] | None:
+        """(hidden with the pending branch added, `norm` of it), or None if nothing is pending.  `inside`: this is
+        `norm`'s own forward that asks."""
         if self.branch is None:
             return None
         mine, branch, behind = self.hidden is hidden, self.branch, self.behind
@@ -969,17 +970,34 @@ class _Carry:
                                "norm read it; the residual carry needs them called back to back "
                                "(fused.enable_residual_carry(model, False) switches it off)")
         if behind is None and norm is not None:
-            return _add_norm(norm, hidden, branch)
-        return _between_blocks(hidden, branch, *(behind or (None, 1.0)), pre=norm)
+            return _add_norm(norm, hidden, branch, inside)
+        return _between_blocks(hidden, branch, *(behind or (None, 1.0)), pre=norm, inside=inside)
 
 
-def _add_norm(norm: nn.Module, x: Tensor, branch: Tensor) -> tuple[Tensor, Tensor]:
-    """(x + branch, norm(x + branch)): one launch where the kernel takes the tensors, else the two steps."""
+def _watched(module: nn.Module, arrivals: bool = True) -> bool:
+    """Whether hooks hang on the calls of this module, so that it has to be called and given what it would get.
+    `arrivals` counts pre-hooks that only wait for its weights and look at no tensor (`looks_at_nothing`)."""
+    pre = module._forward_pre_hooks
+    if pre and not arrivals:
+        pre = [h for h in pre.values() if not getattr(h, "looks_at_nothing", False)]
+    return bool(pre or module._forward_hooks or module._backward_hooks or module._backward_pre_hooks) \
+        or nn.modules.module._has_any_global_hook()
+
+
+def _add_norm(norm: nn.Module, x: Tensor, branch: Tensor, inside: bool = False) -> tuple[Tensor, Tensor]:
+    """(x + branch, norm(x + branch)): one launch where the kernel takes the tensors and nothing hangs on the norm's
+    calls, else the two steps.  `inside`: called by the norm's own forward."""
     w = norm.weight
-    if not hasattr(w, "to_local") and add_rms_norm_supported(x, branch, w):
+    if not hasattr(w, "to_local") and add_rms_norm_supported(x, branch, w) and (inside or not _watched(norm)):
         return add_rms_norm(x, branch, w, norm.variance_epsilon)
     total = x + branch
-    return total, norm(total)
+    return total, norm.forward(total) if inside else norm(total)
+
+
+def _hands_on(layer: nn.Module) -> bool:
+    """Whether a layer may leave its last addition to the next reader: nobody looks at what it returns, nor at what
+    that reader is given."""
+    return not _watched(layer, arrivals=False) and not _watched(layer._prl_reader[0], arrivals=False)
 
 
 def _fused_layer_forward(self: nn.Module, hidden_states: Tensor, attention_mask: Tensor | None = None,
@@ -1004,7 +1022,7 @@ def _fused_layer_forward(self: nn.Module, hidden_states: Tensor, attention_mask:
                                position_embeddings=position_embeddings, **kwargs)
     x, normed = _add_norm(self.post_attention_layernorm, x, branch)
     branch = self.mlp(normed)
-    if carry is None:
+    if carry is None or not _hands_on(self):
         return x + branch
     carry.put(x, branch)
     return x
@@ -1182,12 +1200,14 @@ def _norm_eps(norm: nn.Module) -> float | None:
 
 
 def _between_blocks(x: Tensor, branch: Tensor, post: nn.Module | None, scale: float,
-                    pre: nn.Module | None) -> tuple[Tensor, Tensor]:
-    """(x + scale post(branch), pre of it): one launch where `block_norms` takes the tensors, else step by step."""
+                    pre: nn.Module | None, inside: bool = False) -> tuple[Tensor, Tensor]:
+    """(x + scale post(branch), pre of it): one launch where `block_norms` takes the tensors and nothing hangs on the
+    norms' calls, else step by step.  `inside`: called by `pre`'s own forward."""
     w1, w2 = (None if n is None else n.weight for n in (post, pre))
     forms = {_norm_form(n) for n in (post, pre) if n is not None}
     if len(forms) <= 1 and None not in forms and not any(hasattr(w, "to_local") for w in (w1, w2)) \
-            and block_norms_supported(x, branch, w1, w2):
+            and block_norms_supported(x, branch, w1, w2) \
+            and not any(_watched(n) for n in (post, None if inside else pre) if n is not None):
         e1 = _norm_eps(post) if post is not None else 0.0
         hidden, normed = block_norms(x, branch, w1, w2, scale=scale, eps=e1, pre_eps=_norm_eps(pre) if pre is not None else e1,
                                      weight_offset=forms.pop() if forms else 0.0)
@@ -1197,8 +1217,7 @@ def _between_blocks(x: Tensor, branch: Tensor, post: nn.Module | None, scale: fl
     hidden = x + (branch if scale == 1.0 else branch * scale)
     if pre is None:
         return hidden, hidden
-    plain = getattr(pre, "_prl_torch_forward", pre)  # (the rebound final norm would look for a pending branch)
-    return hidden, plain(hidden)
+    return hidden, pre.forward(hidden) if inside else pre(hidden)
 
 
 def _fused_steps_forward(self: nn.Module, hidden_states: Tensor, *args: Any, **kwargs: Any) -> Tensor:
@@ -1231,7 +1250,7 @@ def _fused_steps_forward(self: nn.Module, hidden_states: Tensor, *args: Any, **k
     factor = lambda name: 1.0 if name is None else float(getattr(self, name))
     x, normed = _between_blocks(x, branch, norm(steps.post1), factor(steps.scale1), norm(steps.pre2))
     branch = self.mlp(normed)
-    if carry is None:
+    if carry is None or not _hands_on(self):
         return _between_blocks(x, branch, norm(steps.post2), factor(steps.scale2), None)[0]
     carry.put(x, branch, (norm(steps.post2), factor(steps.scale2)))
     return x
@@ -1242,7 +1261,7 @@ def enable_residual_carry(model: nn.Module, on: bool = True) -> int:
     to the final norm) instead of adding it itself.  Only for a model whose layers run back to back in one
     process-local forward: not under per-layer activation checkpointing (a re-run layer would not get the branch
     again) nor under per-layer FSDP (its pre-backward hook hangs on the layer's returned tensor, and the MLP's
-    backward can run before it).  Returns the number of layers that carry (0: the model is not shaped for it)."""
+    backward can run before it).  A layer that hooks hang on, or on whose reader they do, adds by itself.  Returns the number of layers that carry (0: the model is not shaped for it)."""
     inner = getattr(model, "model", None)
     layers = list(getattr(inner, "layers", []) or [])
     final = getattr(inner, "norm", None)
@@ -1256,6 +1275,7 @@ def enable_residual_carry(model: nn.Module, on: bool = True) -> int:
     carry = _Carry()
     for i, m in enumerate(layers):
         m._prl_carry, m._prl_first = carry, i == 0
+        m._prl_reader = (layers[i + 1] if i + 1 < len(layers) else final,)  # (in a tuple: not a child module)
     final._prl_carry = carry
     return len(layers)
 
@@ -1263,7 +1283,7 @@ def enable_residual_carry(model: nn.Module, on: bool = True) -> int:
 def _fused_rmsnorm_forward(self: nn.Module, hidden_states: Tensor) -> Tensor:
     carry: _Carry | None = getattr(self, "_prl_carry", None)
     if carry is not None:  # the final norm behind layers that carry their last addition
-        joined = carry.join(hidden_states, self)
+        joined = carry.join(hidden_states, self, inside=True)
         if joined is not None:
             return joined[1]
     weight = self.weight
@@ -1572,7 +1592,7 @@ def unfuse_model(model: nn.Module) -> None:
         if hasattr(module, "_prl_torch_forward"):
             module.forward = module._prl_torch_forward
             del module._prl_torch_forward
-            for attr in ("_prl_qkv", "_prl_carry", "_prl_first", "_prl_steps"):
+            for attr in ("_prl_qkv", "_prl_carry", "_prl_first", "_prl_reader", "_prl_steps"):
                 if hasattr(module, attr):
                     delattr(module, attr)
 

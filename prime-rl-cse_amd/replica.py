@@ -553,6 +553,7 @@ class Replica:
                 for k in which:
                     st.wait_gathered(st.buckets[k])
 
+            hook.looks_at_nothing = True  # (the residual carry goes on past it: `fused._watched`)
             return hook
 
         for module, which in arrival_hooks(self.model, st.params, st.bucket_of):

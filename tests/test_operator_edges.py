@@ -71,3 +71,127 @@ def test_a_norm_of_unknown_form_is_called(post, monkeypatch):
     hidden, normed = fused._between_blocks(x, branch, norm if post else None, 0.5, None if post else norm)
     want = x + 0.5 * (norm(branch) if post else branch)
     assert torch.equal(hidden, want) and torch.equal(normed, want if post else norm(want))
+
+
+def sandwich(name="Glm4"):
+    from tests.test_fuse_families import tiny
+
+    model = tiny(name, num_hidden_layers=2)
+    gen = torch.Generator().manual_seed(1)
+    with torch.no_grad():
+        for p in model.parameters():
+            p.add_(torch.randn(p.shape, generator=gen) * 0.05)
+    return model
+
+
+def stepwise(monkeypatch):
+    """`block_norms` and `add_rms_norm` from elementary operations, so that the fused layers run on the host."""
+    rms = lambda v, w, eps: v * torch.rsqrt((v * v).mean(-1, keepdim=True) + eps) * w
+    calls = []
+
+    def block_norms(x, branch, w1, w2, *, scale, eps, pre_eps, weight_offset):
+        calls.append("block_norms")
+        hidden = x + scale * (branch if w1 is None else rms(branch, w1 + weight_offset, eps))
+        return hidden, None if w2 is None else rms(hidden, w2 + weight_offset, pre_eps)
+
+    def add_rms_norm(x, branch, w, eps):
+        calls.append("add_rms_norm")
+        return x + branch, rms(x + branch, w, eps)
+
+    monkeypatch.setattr(fused, "block_norms_supported", lambda *a, **k: True)
+    monkeypatch.setattr(fused, "block_norms", block_norms)
+    monkeypatch.setattr(fused, "add_rms_norm_supported", lambda *a: True)
+    monkeypatch.setattr(fused, "add_rms_norm", add_rms_norm)
+    return calls
+
+
+def logits(model):
+    ids = torch.arange(2 * 12).view(2, 12) % 160
+    return model(input_ids=ids, position_ids=torch.arange(12).expand(2, 12)).logits
+
+
+def close(a, b):  # fp32, two layers: a norm left out or a hook not run changes values by their own size
+    return bool((a - b).abs().max() <= 2000 * 2.0**-24 * b.abs().max())
+
+
+HOOKS = {
+    "forward": lambda m: m.register_forward_hook(lambda mod, args, out: out * 1.5),
+    "pre": lambda m: m.register_forward_pre_hook(lambda mod, args: (args[0] * 0.5 + 1.0,)),
+    "global": lambda m: torch.nn.modules.module.register_module_forward_hook(
+        lambda mod, args, out: out * 1.5 if mod is m else None),
+}
+
+
+@pytest.mark.parametrize("carry", [False, True])
+@pytest.mark.parametrize("kind", list(HOOKS))
+@pytest.mark.parametrize("name", ["Glm4", "Gemma2", "Olmo2", "Granite", "Qwen3"])
+def test_hooks_on_norms_run(name, kind, carry, monkeypatch):
+    model = sandwich(name)
+    norms = {n: m for n, m in model.named_modules() if n.startswith("model.") and type(m).__name__.endswith("RMSNorm")
+             and "self_attn" not in n}
+    stepwise(monkeypatch)
+    for n, m in norms.items():
+        handle = HOOKS[kind](m)
+        try:
+            want = logits(model)
+            fused.fuse_model(model)
+            try:
+                fused.enable_residual_carry(model, carry)
+                assert close(logits(model), want), n
+            finally:
+                fused.unfuse_model(model)
+        finally:
+            handle.remove()
+        assert not close(logits(model), want), n  # (the hook did change something)
+
+
+@pytest.mark.parametrize("name", ["Glm4", "Granite", "Qwen3"])
+def test_hooks_on_layers_see_whole_hidden_states(name, monkeypatch):
+    model = sandwich(name)
+    calls = stepwise(monkeypatch)
+
+    def look():
+        seen = []
+        handles = []
+        for m in (*model.model.layers, model.model.norm):
+            handles.append(m.register_forward_pre_hook(lambda mod, args: seen.append(args[0].detach().clone())))
+            handles.append(m.register_forward_hook(lambda mod, args, out: seen.append(out.detach().clone())))
+        logits(model)
+        for h in handles:
+            h.remove()
+        return seen
+
+    want = look()
+    fused.fuse_model(model)
+    try:
+        assert fused.enable_residual_carry(model) == 2
+        got = look()
+        assert len(got) == len(want) == 6 and all(close(a, b) for a, b in zip(got, want))
+        # one layer's hook alone leaves the others their carry; a hook that looks at nothing leaves it to all
+        plain = logits(model)
+        calls.clear()
+        logits(model)
+        every = list(calls)
+        hook = lambda mod, args: None
+        hook.looks_at_nothing = True
+        handle = model.model.layers[1].register_forward_pre_hook(hook)
+        calls.clear()
+        assert torch.equal(logits(model), plain) and calls == every
+        handle.remove()
+    finally:
+        fused.unfuse_model(model)
+    assert not hasattr(model.model.layers[0], "_prl_reader")
+
+
+def test_backward_hooks_on_norms_run(monkeypatch):
+    model = sandwich("Glm4")
+    stepwise(monkeypatch)
+    fused.fuse_model(model)
+    try:
+        seen = []
+        for layer in model.model.layers:
+            layer.post_mlp_layernorm.register_full_backward_hook(lambda mod, gi, go: seen.append(tuple(go[0].shape)))
+        logits(model).sum().backward()
+        assert seen == [(2, 12, 64)] * 2
+    finally:
+        fused.unfuse_model(model)
