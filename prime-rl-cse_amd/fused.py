@@ -1526,7 +1526,8 @@ def fuse_model(model: nn.Module) -> dict[str, int]:
         done["lm_head"] = 1
     for module in model.modules():
         name = type(module).__name__
-        is_norm = name.endswith("RMSNorm") and hasattr(module, "weight") and hasattr(module, "variance_epsilon")
+        is_norm = name.endswith("RMSNorm") and hasattr(module, "weight") and hasattr(module, "variance_epsilon") \
+            and _norm_form(module) != 1.0  # (`rms_norm` multiplies by the weight itself)
         if is_norm and not hasattr(module, "_prl_torch_forward"):
             module._prl_torch_forward = module.forward
             module.forward = types.MethodType(_fused_rmsnorm_forward, module)

@@ -195,3 +195,14 @@ def test_backward_hooks_on_norms_run(monkeypatch):
         assert seen == [(2, 12, 64)] * 2
     finally:
         fused.unfuse_model(model)
+
+
+def test_fuse_model_leaves_norms_that_add_one_to_their_weight():
+    class FlaggedRMSNorm(FlaggedNorm):
+        def __init__(self, from_one):
+            super().__init__(from_one)
+            self.variance_epsilon = self.eps
+
+    norms = torch.nn.ModuleList([FlaggedRMSNorm(False), FlaggedRMSNorm(True)])
+    assert fused.fuse_model(norms)["rmsnorm"] == 1
+    assert hasattr(norms[0], "_prl_torch_forward") and not hasattr(norms[1], "_prl_torch_forward")
