@@ -1041,7 +1041,7 @@ def _is_plain_decoder_layer(module: nn.Module) -> bool:
         return False
     if not all(hasattr(module, a) for a in ("input_layernorm", "post_attention_layernorm", "self_attn", "mlp")):
         return False
-    if not all(hasattr(n, "variance_epsilon") and hasattr(n, "weight")
+    if not all(hasattr(n, "variance_epsilon") and hasattr(n, "weight") and _norm_form(n) != 1.0
                for n in (module.input_layernorm, module.post_attention_layernorm)):
         return False
     import inspect

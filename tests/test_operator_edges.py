@@ -206,3 +206,15 @@ def test_fuse_model_leaves_norms_that_add_one_to_their_weight():
     norms = torch.nn.ModuleList([FlaggedRMSNorm(False), FlaggedRMSNorm(True)])
     assert fused.fuse_model(norms)["rmsnorm"] == 1
     assert hasattr(norms[0], "_prl_torch_forward") and not hasattr(norms[1], "_prl_torch_forward")
+
+
+def test_a_plain_layer_with_norms_that_add_one_is_left_alone():
+    layer = sandwich("Qwen3").model.layers[0]
+    assert fused._is_plain_decoder_layer(layer)
+
+    class FromOneRMSNorm(type(layer.input_layernorm)):
+        def forward(self, x):
+            return x * torch.rsqrt((x * x).mean(-1, keepdim=True) + self.variance_epsilon) * (1.0 + self.weight)
+
+    layer.post_attention_layernorm.__class__ = FromOneRMSNorm
+    assert not fused._is_plain_decoder_layer(layer)
