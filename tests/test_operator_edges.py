@@ -209,8 +209,8 @@ def test_fuse_model_leaves_norms_that_add_one_to_their_weight():
 
 
 def test_a_plain_layer_with_norms_that_add_one_is_left_alone():
-    layer = sandwich("Qwen3").model.layers[0]
-    assert fused._is_plain_decoder_layer(layer)
+    plain, layer = sandwich("Qwen3").model.layers
+    assert fused._is_plain_decoder_layer(plain)
 
     class FromOneRMSNorm(type(layer.input_layernorm)):
         def forward(self, x):
