@@ -24,6 +24,7 @@ from typing import Any
 
 import torch
 from torch import Tensor, nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _capi as C
@@ -39,6 +40,13 @@ def _first_derivative(backward: Any) -> Any:
         return once(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return run
+
+
+def _through_autograd(*tensors: Tensor | None) -> bool:
+    """Whether a call on these goes through its autograd function: a gradient is wanted, or a forward-mode level is open
+    (the function refuses dual tensors; a launch by itself would drop their tangents)."""
+    return forward_ad._current_level >= 0 or (
+        torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
 
 
 def _row_layout(x: Tensor):
@@ -348,7 +356,7 @@ def block_norms(x: Tensor, branch: Tensor, post_weight: Tensor | None = None, pr
     w2 = None if pre_weight is None else pre_weight.contiguous()
     args = (x, branch, w1, w2, gate, kind, float(scale), float(weight_offset), float(eps),
             float(eps if pre_eps is None else pre_eps))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, branch, w1, w2, gate)):
+    if _through_autograd(x, branch, w1, w2, gate):
         hidden, normed = _BlockNorms.apply(*args)
     else:
         hidden, normed = torch.empty_like(x), None if w2 is None else torch.empty_like(x)
@@ -695,7 +703,7 @@ def rope_at_positions(q: Tensor, k: Tensor | None, position_ids: Tensor, inv_fre
             f"{tuple(position_ids.shape)} {position_ids.dtype}, inv_freq {tuple(inv_freq.shape)} {inv_freq.dtype}")
     pos = position_ids if position_ids.ndim == 2 else position_ids.unsqueeze(0)
     inv_freq = inv_freq.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if _through_autograd(q, k):
         return _RopePositions.apply(q, k, pos, inv_freq, bool(interleaved), float(attention_scaling))
     return _launch_rope_positions(q, k, pos, inv_freq, bool(interleaved), float(attention_scaling), False)
 

@@ -10,6 +10,15 @@ import prime_rl_cse_amd as prl  # noqa: F401
 from prime_rl_cse_amd import fused
 
 
+@pytest.fixture(autouse=True)
+def one_thread():
+    """Tiny tensors: handing them to threads takes longer than the work."""
+    threads = torch.get_num_threads()
+    torch.set_num_threads(1)
+    yield
+    torch.set_num_threads(threads)
+
+
 class FlaggedNorm(torch.nn.Module):
     """An RMSNorm whose instances say for themselves whether the weight is a distance from one."""
 
@@ -218,3 +227,27 @@ def test_a_plain_layer_with_norms_that_add_one_is_left_alone():
 
     layer.post_attention_layernorm.__class__ = FromOneRMSNorm
     assert not fused._is_plain_decoder_layer(layer)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(grad, monkeypatch):
+    """Neither operator has one: a call on dual tensors fails instead of dropping the tangents."""
+    import torch.autograd.forward_ad as fa
+
+    monkeypatch.setattr(fused, "block_norms_supported", lambda *a: True)
+    monkeypatch.setattr(fused, "_launch_block_norms", lambda *a: None)
+    monkeypatch.setattr(fused, "rope_at_positions_supported", lambda *a: True)
+    monkeypatch.setattr(fused, "_launch_rope_positions", lambda q, k, *a: (q.clone(), None if k is None else k.clone()))
+    x, w, gate = torch.randn(3, 8), torch.randn(8), torch.rand(3, 1)
+    q, pos, freq = torch.randn(1, 2, 3, 8), torch.arange(3), torch.ones(4)
+    norms = lambda *t: fused.block_norms(*t[:4], gate=t[4])
+    rope = lambda *t: fused.rope_at_positions(*t, pos, freq)
+    with torch.set_grad_enabled(grad), fa.dual_level():
+        for call, args in ((norms, [x, x.clone(), w, w.clone(), gate]), (rope, [q, q.clone()])):
+            for i, t in enumerate(args):
+                dual = list(args)
+                dual[i] = fa.make_dual(t, torch.ones_like(t))
+                with pytest.raises(NotImplementedError):
+                    call(*dual)
+            call(*args)  # (a level that none of the inputs takes part in)
+        rope(q, None)
