@@ -232,6 +232,13 @@ def _pitched(x: Tensor, h: int) -> Tensor:
     return x
 
 
+def _fresh_rows(x: Tensor) -> Tensor:
+    """Memory for rows like x's, h apart.  (`empty_like` is the cheapest call, but of rows that overlap it makes rows one
+    element apart.)"""
+    out = torch.empty_like(x)
+    return out if out.stride(0) == x.shape[1] else torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 def _gate_rows(gate: Tensor, lead: tuple[int, ...], h: int) -> tuple[int, Tensor]:
     """(kind, the gate as the kernels read it): [h], one value per row, [rows, h], or one value."""
     if gate.shape == (*lead, h):
@@ -270,9 +277,8 @@ class _BlockNorms(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, branch: Tensor, w_post: Tensor | None, w_pre: Tensor | None, gate: Tensor | None,
                 kind: int, scale: float, offset: float, eps_post: float, eps_pre: float):
-        # (empty_like: rows of another pitch are given h, the cheaper call otherwise)
-        hidden = torch.empty_like(x)
-        normed = None if w_pre is None else torch.empty_like(x)
+        hidden = _fresh_rows(x)
+        normed = None if w_pre is None else _fresh_rows(x)
         rstd = torch.empty(2 * x.shape[0], dtype=torch.float32, device=x.device)  # of the branch, then of the sum
         _launch_block_norms(x, branch, w_post, w_pre, gate, kind, scale, offset, eps_post, eps_pre, hidden, normed, rstd)
         ctx.save_for_backward(x, branch, w_post, w_pre, gate, rstd)
@@ -295,7 +301,7 @@ class _BlockNorms(torch.autograd.Function):
         gh = None if gh is None else _pitched(gh, h)
         gy = None if gy is None else _pitched(gy, h)
         need = ctx.needs_input_grad
-        gx, gb = torch.empty_like(x), torch.empty_like(x)
+        gx, gb = _fresh_rows(x), _fresh_rows(x)
         g1 = torch.empty_like(w_post) if w_post is not None and need[2] else None
         g2 = torch.empty_like(w_pre) if w_pre is not None and need[3] else None
         gg = torch.empty(gate.shape, dtype=x.dtype, device=dev) if gate is not None and need[4] else None
@@ -359,7 +365,7 @@ def block_norms(x: Tensor, branch: Tensor, post_weight: Tensor | None = None, pr
     if _through_autograd(x, branch, w1, w2, gate):
         hidden, normed = _BlockNorms.apply(*args)
     else:
-        hidden, normed = torch.empty_like(x), None if w2 is None else torch.empty_like(x)
+        hidden, normed = _fresh_rows(x), None if w2 is None else _fresh_rows(x)
         _launch_block_norms(*args, hidden, normed, None)
     if len(shape) != 2:
         hidden, normed = hidden.view(shape), None if normed is None else normed.view(shape)
@@ -639,6 +645,8 @@ def _launch_rope_positions(q: Tensor | None, k: Tensor | None, pos: Tensor, inv_
             args += [None, None, None, 0]
             continue
         out = torch.empty_like(x)
+        if out.stride(3) != 1:  # (a guess at the layout of memory that overlaps)
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
         outs.append(out)
         args += [x.data_ptr(), out.data_ptr(), _strides6(x, out), x.shape[1]]
     if 0 in (b, t) or args[3] + args[7] == 0:

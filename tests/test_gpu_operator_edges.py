@@ -1,0 +1,53 @@
+"""Calls at the edges of the operators of the fused layers and of clipping, on the GPU: inputs that overlap in memory,
+hooks in the package's own step.  The host's side is tests/test_operator_edges.py."""
+
+import pytest
+import torch
+
+import prime_rl_cse_amd as prl  # noqa: F401
+from prime_rl_cse_amd import fused
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows, h, strides", [(5, 8, (1, 1)), (4, 96, (1, 1)), (300, 72, (1, 1)), (7, 1000, (8, 1)),
+                                              (3, 5000, (0, 1))])
+def test_norms_of_rows_that_overlap(rows, h, strides, dtype):
+    """Windows of one run of memory give what their copies give, bit for bit, both ways."""
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    base = torch.randn(20000, generator=gen, device=DEV).to(dtype)
+    make = lambda at, copied: base[at:].as_strided((rows, h), strides).clone(memory_format=torch.contiguous_format) \
+        if copied else base[at:].as_strided((rows, h), strides)
+    w1, w2, gh, gy = (torch.randn(n, generator=gen, device=DEV).to(dtype) for n in ((h,), (h,), (rows, h), (rows, h)))
+    results = []
+    for copied in (False, True):
+        x, b, g = (make(at, copied).requires_grad_(True) for at in (0, 16, 32))
+        with torch.no_grad():
+            bare = fused.block_norms(x, b, w1, w2, gate=g)
+        out = fused.block_norms(x, b, w1, w2, gate=g)
+        results.append([*bare, *out, *torch.autograd.grad(out, [x, b, g], [gh, gy])])
+        assert results[-1][0].stride() == (h, 1)
+    for got, want in zip(*results):
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("strides", [(60, 30, 1, 1), (0, 1, 0, 1), (1, 1, 1, 1), (64, 0, 32, 1), (1, 400, 16, 1)])
+def test_rotation_of_heads_that_overlap(strides, dtype, interleaved):
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    base = torch.randn(20000, generator=gen, device=DEV).to(dtype)
+    freq, _ = fused.rope_frequencies(16, device=DEV)
+    pos = torch.arange(9, device=DEV) * 1000
+    results = []
+    for copied in (False, True):
+        q, k, gq, gk = (base[at:].as_strided((3, n, 9, 16), strides) for at, n in ((0, 4), (64, 2), (128, 4), (192, 2)))
+        if copied:
+            q, k, gq, gk = (t.clone(memory_format=torch.contiguous_format) for t in (q, k, gq, gk))
+        q, k = q.requires_grad_(True), k.requires_grad_(True)
+        out = fused.rope_at_positions(q, k, pos, freq, interleaved=interleaved)
+        results.append([*out, *torch.autograd.grad(out, [q, k], [gq, gk])])
+    for got, want in zip(*results):
+        assert torch.equal(got, want)

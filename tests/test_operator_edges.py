@@ -251,3 +251,45 @@ def test_forward_mode_derivatives_are_refused(grad, monkeypatch):
                     call(*dual)
             call(*args)  # (a level that none of the inputs takes part in)
         rope(q, None)
+
+
+WINDOWS = [(1, 1), (0, 1), (3, 1), (8, 1), (12, 1), (1, 0), (2, 3)]  # strides of 5 rows of 8 out of one run of memory
+
+
+@pytest.mark.parametrize("strides", WINDOWS)
+def test_outputs_of_overlapping_rows_lie_row_by_row(strides, monkeypatch):
+    """Inputs that are windows of one run of memory: the kernels write rows of their own pitch."""
+    seen = []
+
+    def run(fn, name, dev, *args):
+        seen.append(name)
+
+    monkeypatch.setattr(fused.C, "run", run)
+    monkeypatch.setattr(fused.C, "stream_ptr", lambda dev: 0)
+    monkeypatch.setattr(fused, "block_norms_supported", lambda *a: True)
+    base = torch.randn(100)
+    x, b = (base[i:].as_strided((5, 8), strides) for i in (0, 1))
+    w = torch.ones(8)
+    for t in fused.block_norms(x, b, w, w):
+        assert t.stride() == (8, 1)
+    out = fused.block_norms(x.requires_grad_(True), b, w, w)
+    for t in (*out, *torch.autograd.grad(out, [x], [torch.ones(5, 8)] * 2)):
+        assert t.stride() == (8, 1)
+    assert seen == ["prl_block_norms_fwd"] * 2 + ["prl_block_norms_bwd"]
+
+
+@pytest.mark.parametrize("strides", [(60, 30, 1, 1), (0, 1, 0, 1), (1, 40, 8, 1), (0, 0, 0, 1), (1, 1, 1, 1), (80, 8, 16, 1),
+                                     (90, 40, 8, 0), (90, 45, 9, 1)])
+def test_rotated_heads_of_overlapping_memory_lie_along_the_head(strides, monkeypatch):
+    monkeypatch.setattr(fused.C, "run", lambda *a: None)
+    monkeypatch.setattr(fused.C, "stream_ptr", lambda dev: 0)
+    q = torch.randn(400).as_strided((3, 2, 5, 8), strides)
+    for inverse in (False, True):
+        qo, ko = fused._launch_rope_positions(q, q, torch.arange(5)[None], torch.ones(4), False, 1.0, inverse)
+        for t in (qo, ko):
+            assert t.stride(3) == 1
+            span = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+            assert span == t.numel() and t.untyped_storage().nbytes() >= 4 * span  # dense: no two elements in one place
+    dense = torch.randn(3, 5, 2, 8).transpose(1, 2)
+    assert fused._launch_rope_positions(dense, None, torch.arange(5)[None], torch.ones(4), False, 1.0, False)[0].stride() == \
+        dense.stride()  # layouts of dense inputs are kept
