@@ -143,17 +143,27 @@ def _is_one_run(g: torch.Tensor) -> bool:
     return True
 
 
+def _overlap(at: np.ndarray, size: np.ndarray) -> bool:
+    """Whether any two runs of `size` bytes at these addresses share memory (empty runs share none)."""
+    at, size = at[size > 0], size[size > 0]
+    order = np.argsort(at)
+    return bool(((at + size)[order[:-1]] > at[order[1:]]).any())
+
+
 def clip_grad_norm_supported(grads: list[torch.Tensor]) -> bool:
-    """Whether `clip_grad_norm_` takes these gradients: bf16 or fp32, each one run of memory, on one HIP device, plain or
-    DTensors of one mesh that are sharded or replicated alike."""
+    """Whether `clip_grad_norm_` takes these gradients: bf16 or fp32, each one run of memory and no two the same, on one
+    HIP device, plain or DTensors of one mesh that are sharded or replicated alike."""
     if not grads:
         return True
     if _sharding(grads) is None:
         return False
     parts = _local_parts(grads)
     index = set(map(torch.Tensor.get_device, parts))
-    return len(index) == 1 and index != {-1} and set(map(_DTYPE, parts)) <= _TYPES \
-        and all(g.layout is torch.strided and _is_one_run(g) for g in parts)
+    if len(index) != 1 or index == {-1} or not set(map(_DTYPE, parts)) <= _TYPES \
+            or not all(g.layout is torch.strided and _is_one_run(g) for g in parts):
+        return False
+    at = np.array(list(map(torch.Tensor.data_ptr, parts)), dtype=np.int64)
+    return not _overlap(at, np.array([g.numel() * g.element_size() for g in parts], dtype=np.int64))
 
 
 _GRAD, _DTYPE = operator.attrgetter("grad"), operator.attrgetter("dtype")
@@ -183,10 +193,8 @@ def _pieces(grads: list[torch.Tensor], in_place: bool) -> np.ndarray:
     if len(table) > 1:
         size = table["n"] * (4 - 2 * table["dtype"])
         at = table["x"]
-        if in_place:
-            order = np.argsort(at)
-            if ((at + size)[order[:-1]] > at[order[1:]]).any():
-                raise ValueError("clip_grad_norm_: two gradients share memory (a parameter given twice?)")
+        if in_place and _overlap(at, size):
+            raise ValueError("clip_grad_norm_: two gradients share memory (a parameter given twice?)")
         first = np.flatnonzero(np.r_[True, ((at + size)[:-1] != at[1:]) | (table["dtype"][:-1] != table["dtype"][1:])])
         if len(first) < len(table):
             n = np.add.reduceat(table["n"], first)

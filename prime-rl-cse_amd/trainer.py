@@ -616,6 +616,14 @@ def restore_row_starts(rows: JoinedRows, mb: dict[str, Any], aux: dict[str, Tens
     return sums[: len(rows.lengths)]
 
 
+def _clip(parameters: Any, max_norm: float) -> Tensor:
+    """Gradient clipping on the package's kernels where they take the gradients (`optim.clip_grad_norm_supported`), else
+    by torch's function."""
+    params = [prm for prm in parameters if prm.grad is not None]
+    clip = clip_grad_norm_ if clip_grad_norm_supported([prm.grad for prm in params]) else torch.nn.utils.clip_grad_norm_
+    return clip(params, max_norm)
+
+
 def train_step(model: nn.Module, optimizer: torch.optim.Optimizer, micro_batches: list[MicroBatch],
                loss_config: LossConfig, max_norm: float = 1.0, device: torch.device | str = "cuda",
                scheduler: Any = None, samples: int | None = None,
@@ -743,9 +751,7 @@ def train_step(model: nn.Module, optimizer: torch.optim.Optimizer, micro_batches
         for prm in model.parameters():
             if prm.requires_grad and prm.grad is None:
                 prm.grad = torch.zeros_like(prm)
-    params = [prm for prm in model.parameters() if prm.grad is not None]
-    clip = clip_grad_norm_ if clip_grad_norm_supported([prm.grad for prm in params]) else torch.nn.utils.clip_grad_norm_
-    grad_norm = clip(params, max_norm)
+    grad_norm = _clip(model.parameters(), max_norm)
     if hasattr(grad_norm, "full_tensor"):
         grad_norm = grad_norm.full_tensor()
     optimizer.step()

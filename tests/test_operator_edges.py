@@ -293,3 +293,37 @@ def test_rotated_heads_of_overlapping_memory_lie_along_the_head(strides, monkeyp
     dense = torch.randn(3, 5, 2, 8).transpose(1, 2)
     assert fused._launch_rope_positions(dense, None, torch.arange(5)[None], torch.ones(4), False, 1.0, False)[0].stride() == \
         dense.stride()  # layouts of dense inputs are kept
+
+
+def on_device(monkeypatch):
+    """Host gradients pass for a device's, so that what is said about their memory can be asked here."""
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+
+
+def test_gradients_that_share_memory_are_not_supported(monkeypatch):
+    from prime_rl_cse_amd import optim
+
+    on_device(monkeypatch)
+    flat = torch.randn(40)
+    apart = [flat[:10], flat[10:20], flat[25:], torch.randn(3).bfloat16(), flat[5:5]]
+    assert optim.clip_grad_norm_supported(apart) and optim.clip_grad_norm_supported([])
+    for shared in ([flat[:10], flat[9:12]], [flat, flat], [*apart, flat[12:13]], [flat[8:12], *apart]):
+        assert not optim.clip_grad_norm_supported(shared)
+        with pytest.raises(ValueError):
+            optim._pieces(shared, True)
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_a_step_with_gradients_that_share_memory_clips_by_torch(shared, monkeypatch):
+    """`train_step` hands to the package's clipping only what that takes."""
+    from prime_rl_cse_amd import trainer as T
+
+    on_device(monkeypatch)
+    flat = torch.randn(12)
+    params = [torch.nn.Parameter(torch.zeros(4)) for _ in range(2)]
+    params[0].grad, params[1].grad = flat[:4], (flat[3:7] if shared else flat[4:8])
+    taken = []
+    monkeypatch.setattr(T, "clip_grad_norm_", lambda p, m: taken.append("package") or torch.tensor(1.0))
+    monkeypatch.setattr(torch.nn.utils, "clip_grad_norm_", lambda p, m: taken.append("torch") or torch.tensor(1.0))
+    T._clip(params, 1.0)
+    assert taken == ["torch" if shared else "package"]
