@@ -642,6 +642,8 @@ extern "C" int prl_block_norms_bwd(const void* x, int64_t x_stride, const void* 
                     {x, branch, w_post, w_pre, gate, g_hidden, g_normed, gx, g_branch, g_w_post, g_w_pre, g_gate},
                     {gx_stride, g_branch_stride, gate_kind == PRL_GATE_FULL && g_gate ? g_gate_stride : H});
   if (rc != PRL_OK) return rc;
+  // (also without a row: the launch that leaves sums of zero reads it)
+  PRL_REQUIRE(gate_kind != PRL_GATE_CHANNEL || gate, "block_norms_bwd: a gate per channel must not be NULL");
   PRL_REQUIRE(gate_kind != PRL_GATE_TOKEN || !g_gate || g_gate_stride >= 1,
               "block_norms_bwd: the row stride of a token gate's gradient must be >= 1");
   PRL_REQUIRE(!g_w_post || w_post, "block_norms_bwd: g_w_post without w_post");

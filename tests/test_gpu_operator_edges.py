@@ -51,3 +51,14 @@ def test_rotation_of_heads_that_overlap(strides, dtype, interleaved):
         results.append([*out, *torch.autograd.grad(out, [q, k], [gq, gk])])
     for got, want in zip(*results):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("gate", [None, "one", "channel", "token", "full"])
+def test_no_rows_with_every_gate(gate):
+    shape = {None: None, "one": (), "channel": (48,), "token": (0, 1), "full": (0, 48)}[gate]
+    x = torch.empty(0, 48, device=DEV, requires_grad=True)
+    w, g = torch.ones(48, device=DEV, requires_grad=True), None if shape is None else torch.ones(shape, device=DEV)
+    leaves = [x, w] if g is None else [x, w, g.requires_grad_(True)]
+    out = fused.block_norms(x, x, w, w, gate=g)
+    for grad, leaf in zip(torch.autograd.grad(out, leaves, [torch.empty(0, 48, device=DEV)] * 2), leaves):
+        assert grad.shape == leaf.shape and not bool(grad.any())

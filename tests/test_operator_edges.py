@@ -327,3 +327,17 @@ def test_a_step_with_gradients_that_share_memory_clips_by_torch(shared, monkeypa
     monkeypatch.setattr(torch.nn.utils, "clip_grad_norm_", lambda p, m: taken.append("torch") or torch.tensor(1.0))
     T._clip(params, 1.0)
     assert taken == ["torch" if shared else "package"]
+
+
+def test_no_rows_and_no_gate_is_refused():
+    """The sums over no rows are still formed by a launch, which reads a gate per channel once."""
+    from prime_rl_cse_amd import _capi as C
+
+    lib, one, none = C.load(), 16, None
+    bwd = lambda rows: lib.prl_block_norms_bwd(one, 16, one, 16, one, one, C.GATE_CHANNEL, none, 16, 1.0, 0.0, one, one, none,
+                                               0, one, 16, one, 16, one, 16, one, one, none, 16, 0, rows, 16, one, 1 << 20,
+                                               none)
+    assert bwd(2) == -1 and bwd(0) == -1
+    # without a row and without a launch no gate is read
+    assert lib.prl_block_norms_fwd(one, 16, one, 16, one, one, C.GATE_CHANNEL, none, 0, 1.0, 0.0, 1e-6, 1e-6, one, 16, one, 16,
+                                   none, none, 0, 0, 16, none) == 0
