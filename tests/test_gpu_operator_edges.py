@@ -6,6 +6,7 @@ import torch
 
 import prime_rl_cse_amd as prl  # noqa: F401
 from prime_rl_cse_amd import fused
+from tests.test_gpu_block_norms import E1, E2, HALF_STEP, U, bounds
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -15,22 +16,26 @@ DEV = "cuda:0"
 @pytest.mark.parametrize("rows, h, strides", [(5, 8, (1, 1)), (4, 96, (1, 1)), (300, 72, (1, 1)), (7, 1000, (8, 1)),
                                               (3, 5000, (0, 1))])
 def test_norms_of_rows_that_overlap(rows, h, strides, dtype):
-    """Windows of one run of memory give what their copies give, bit for bit, both ways."""
+    """Windows of one run of memory.  Copies of them may take another form of the kernel, which adds a row up in another
+    order, so both are held to the definition, within the roundings that `test_gpu_block_norms.check` counts (no sums over
+    rows here)."""
     gen = torch.Generator(device=DEV).manual_seed(0)
     base = torch.randn(20000, generator=gen, device=DEV).to(dtype)
     make = lambda at, copied: base[at:].as_strided((rows, h), strides).clone(memory_format=torch.contiguous_format) \
         if copied else base[at:].as_strided((rows, h), strides)
     w1, w2, gh, gy = (torch.randn(n, generator=gen, device=DEV).to(dtype) for n in ((h,), (h,), (rows, h), (rows, h)))
-    results = []
     for copied in (False, True):
         x, b, g = (make(at, copied).requires_grad_(True) for at in (0, 16, 32))
         with torch.no_grad():
-            bare = fused.block_norms(x, b, w1, w2, gate=g)
-        out = fused.block_norms(x, b, w1, w2, gate=g)
-        results.append([*bare, *out, *torch.autograd.grad(out, [x, b, g], [gh, gy])])
-        assert results[-1][0].stride() == (h, 1)
-    for got, want in zip(*results):
-        assert torch.equal(got, want)
+            bare = fused.block_norms(x, b, w1, w2, gate=g, eps=E1, pre_eps=E2)
+        out = fused.block_norms(x, b, w1, w2, gate=g, eps=E1, pre_eps=E2)
+        got = dict(zip("hyxbg", (*out, *torch.autograd.grad(out, [x, b, g], [gh, gy]))))
+        assert all(t.stride() == (h, 1) for t in got.values())
+        assert torch.equal(bare[0], got["h"]) and torch.equal(bare[1], got["y"])
+        want, mag = bounds(dict(x=x, b=b, w1=w1, w2=w2, g=g, gh=gh, gy=gy), 1.0, 0.0, rows)
+        for name, t in got.items():
+            tol = HALF_STEP[dtype] * want[name].abs() * (1 + 2.0**-10) + (64 if name in "hy" else 160) * U * mag[name] + 1e-30
+            assert bool(((t.double() - want[name]).abs() <= tol).all()), (name, copied)
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
