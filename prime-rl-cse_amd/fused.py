@@ -1163,6 +1163,8 @@ def _layer_steps(module: nn.Module) -> _LayerSteps | None:
         return None
     if steps.post1 is None and steps.post2 is None and steps.scale1 is None and steps.scale2 is None:
         return None
+    if any(not isinstance(getattr(module, n, None), (int, float)) for n in (steps.scale1, steps.scale2) if n):
+        return None  # (a tensor may be learned)
     if any(_norm_form(getattr(module, n)) is None for n in (steps.pre1, steps.post1, steps.pre2, steps.post2) if n):
         return None
     return steps

@@ -341,3 +341,14 @@ def test_no_rows_and_no_gate_is_refused():
     # without a row and without a launch no gate is read
     assert lib.prl_block_norms_fwd(one, 16, one, 16, one, one, C.GATE_CHANNEL, none, 0, 1.0, 0.0, 1e-6, 1e-6, one, 16, one, 16,
                                    none, none, 0, 0, 16, none) == 0
+
+
+def test_a_learned_factor_on_the_residual_leaves_the_layer_alone():
+    """The kernel's factor is a number: a tensor's gradient would be lost."""
+    layer = sandwich("Granite").model.layers[0]
+    assert fused._layer_steps(layer) is not None
+    layer.residual_multiplier = torch.nn.Parameter(torch.tensor(0.5))
+    assert fused._layer_steps(layer) is None
+    layer = sandwich("Granite").model.layers[0]
+    layer.residual_multiplier = torch.tensor(0.5)
+    assert fused._layer_steps(layer) is None
