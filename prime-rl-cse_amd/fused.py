@@ -501,43 +501,58 @@ def _family_rope(original: Any, kind: str) -> Any:
 def _rope_kind(home: Any, model: nn.Module) -> tuple[str, list[nn.Module]] | None:
     """How a family's `apply_rotary_pos_emb` pairs the dimensions of a head, found by what it does to a small host
     tensor, and the rotary modules to tag (none for whole heads in the half layout, which have their tables); None for
-    a function that does something else."""
-    import copy
-
-    original = home.apply_rotary_pos_emb
+    a function that does something else.  Every rotary module is tried by itself; one whose tables are made another way
+    is not tagged."""
     modules = [m for m in model.modules() if type(m).__name__.endswith("RotaryEmbedding")
-               and isinstance(getattr(m, "inv_freq", None), Tensor)]
+               and isinstance(getattr(m, "inv_freq", None), Tensor) and not m.inv_freq.is_meta]
     config = getattr(model, "config", None)
     heads = getattr(config, "num_attention_heads", None)
     size = getattr(config, "head_dim", None) or (config.hidden_size // heads if heads else None)
-    if not modules or modules[0].inv_freq.is_meta or size is None:
+    if not modules or size is None:
         try:  # no tables to be had: the pairs are told by the helper that these families have
-            turned = home.rotate_half(torch.arange(4.0)).tolist()
+            turned = home.rotate_half(torch.arange(4.0, device="cpu")).tolist()
         except Exception:
             return "half", []
         return ("half", []) if turned == [-2.0, -3.0, 0.0, 1.0] else None
-    rotary = copy.deepcopy(modules[0])
+    kinds = [_probe_rotary(home.apply_rotary_pos_emb, m, size) for m in modules]
+    kind = next((k for k in kinds if k is not None), None)
+    if kind is None:
+        return None
+    own = lambda m: getattr(m.__dict__.get("_prl_torch_forward", m.forward), "__func__", None) is type(m).forward
+    return kind, [m for m, k in zip(modules, kinds) if k == kind and own(m)
+                  and not (kind == "half" and size == 2 * m.inv_freq.numel())]
+
+
+def _probe_rotary(rotate: Any, module: nn.Module, size: int) -> str | None:
+    """"half" or "interleaved", if `rotate` with this rotary module's tables turns a head of `size` (or one turned as a
+    whole) that way, by position times the module's `inv_freq`; None otherwise."""
+    import copy
+
+    rotary = copy.deepcopy(module)
     rotary.forward = types.MethodType(type(rotary).forward, rotary)
     rotary = rotary.cpu().float()
     gen = torch.Generator().manual_seed(0)
-    pos = torch.tensor([[3, 4, 5, 11, 2]])
+    randn = lambda *shape: torch.randn(shape, generator=gen, dtype=torch.float32, device="cpu")
+    pos = torch.tensor([[3, 4, 5, 11, 2]], device="cpu")
     r = 2 * rotary.inv_freq.numel()
     for d in dict.fromkeys((size, r)):
-        q, k = torch.randn(1, 2, 5, d, generator=gen), torch.randn(1, 1, 5, d, generator=gen)
+        q, k = randn(1, 2, 5, d), randn(1, 1, 5, d)
         try:
             with torch.no_grad():
                 cos, sin = rotary(q, pos)
-                got = original(q, k, cos, sin)[0]
+                got = rotate(q, k, cos, sin)[0]
         except Exception:
             continue
         theta = (pos[..., None] * rotary.inv_freq)[:, None]
         c, s = theta.cos() * getattr(rotary, "attention_scaling", 1.0), theta.sin() * getattr(rotary, "attention_scaling", 1.0)
         for kind in ("half", "interleaved"):
             u, v = (q[..., : r // 2], q[..., r // 2 : r]) if kind == "half" else (q[..., 0:r:2], q[..., 1:r:2])
+            if u.shape[-1] != r // 2 or v.shape[-1] != r // 2:
+                continue
             a, b = u * c - v * s, v * c + u * s
             want = torch.cat([a, b], -1) if kind == "half" else torch.stack([a, b], -1).flatten(-2)
             if got.shape == q.shape and torch.allclose(got, torch.cat([want, q[..., r:]], -1), rtol=1e-4, atol=1e-5):
-                return kind, [] if kind == "half" and size == r else modules
+                return kind
     return None
 
 

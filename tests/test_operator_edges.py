@@ -352,3 +352,54 @@ def test_a_learned_factor_on_the_residual_leaves_the_layer_alone():
     layer = sandwich("Granite").model.layers[0]
     layer.residual_multiplier = torch.tensor(0.5)
     assert fused._layer_steps(layer) is None
+
+
+class OtherRotaryEmbedding(torch.nn.Module):
+    """Tables of another kind, from a length: what a vision tower keeps beside the decoder's."""
+
+    def __init__(self):
+        super().__init__()
+        self.register_buffer("inv_freq", torch.rand(4))
+
+    def forward(self, length):
+        return torch.outer(torch.arange(length), self.inv_freq)
+
+
+@pytest.mark.parametrize("first", [False, True])
+def test_only_rotary_modules_that_do_what_was_found_are_tagged(first):
+    """Each module is tried by itself: another one in the model keeps its own forward."""
+    import sys
+
+    model = sandwich("Glm4")
+    rotary, other = model.model.rotary_emb, OtherRotaryEmbedding()
+    doubled = copy.deepcopy(rotary)  # the same class, another relation between tables and frequencies
+    doubled.register_buffer("inv_freq", rotary.inv_freq.clone())
+    doubled.forward = lambda x, pos: tuple(2 * t for t in type(rotary).forward(doubled, x, pos))
+    extra = torch.nn.ModuleList([other, doubled])
+    if first:
+        model._modules = {"extra": extra, **model._modules}
+    else:
+        model.extra = extra
+    kind, tagged = fused._rope_kind(sys.modules[type(model).__module__], model)
+    assert kind == "interleaved" and tagged == [rotary]
+    fused.fuse_model(model)
+    try:
+        assert other(3).shape == (3, 4)
+        cos, _ = doubled(torch.zeros(1, 1, 3, 16), torch.arange(3)[None])
+        assert not hasattr(cos, "_prl_rope")
+        assert hasattr(rotary(torch.zeros(1, 1, 3, 16), torch.arange(3)[None])[0], "_prl_rope")
+    finally:
+        fused.unfuse_model(model)
+
+
+def test_pairs_are_found_under_other_defaults():
+    import sys
+
+    model = sandwich("Glm4")
+    before = torch.get_default_dtype()
+    try:
+        torch.set_default_dtype(torch.bfloat16)
+        kind, tagged = fused._rope_kind(sys.modules[type(model).__module__], model)
+    finally:
+        torch.set_default_dtype(before)
+    assert kind == "interleaved" and tagged == [model.model.rotary_emb]
