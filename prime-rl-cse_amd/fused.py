@@ -485,7 +485,9 @@ def _family_rope(original: Any, kind: str) -> Any:
     from a tagged rotary module, the family's own function for everything else."""
 
     def rotate(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, *args: Any, **kwargs: Any):
-        if not args and not kwargs or (kwargs == {"unsqueeze_dim": 1} and not args) or (args == (1,) and not kwargs):
+        given = args or tuple(kwargs.values())  # (a tensor's == is a tensor: types first)
+        if not given or (len(args) + len(kwargs) == 1 and type(given[0]) is int and given[0] == 1
+                         and (args or "unsqueeze_dim" in kwargs)):
             source = getattr(cos, "_prl_rope", None)
             if source is None or not source.stands(cos, sin):
                 if kind == "half" and rope_supported(q, k, cos, sin):

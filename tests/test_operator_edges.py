@@ -403,3 +403,31 @@ def test_pairs_are_found_under_other_defaults():
     finally:
         torch.set_default_dtype(before)
     assert kind == "interleaved" and tagged == [model.model.rotary_emb]
+
+
+def rotated_by(monkeypatch, kind="interleaved"):
+    taken = []
+    monkeypatch.setattr(fused, "rope_at_positions_supported", lambda *a: True)
+    monkeypatch.setattr(fused, "rope_at_positions", lambda q, k, *a, **kw: taken.append("positions") or (q, k))
+    return taken, fused._family_rope(lambda q, k, cos, sin, *a, **kw: taken.append("tables") or (q, k), kind)
+
+
+def tables(model=None, dtype=torch.float32, t=5):
+    rotary = (model or sandwich("Glm4")).model.rotary_emb
+    rotary._prl_torch_forward = rotary.forward
+    return fused._tagged_rotary_forward(rotary, torch.zeros(1, 2, t, 16, dtype=dtype), torch.arange(t)[None])
+
+
+@pytest.mark.parametrize("extra", [(torch.arange(5)[None],), (2,), (None,), (1.0,), (True,), (2, 1)])
+def test_other_arguments_go_to_the_family_s_function(extra, monkeypatch):
+    """Positions behind the tables, another axis for the heads: only the plain call is taken over."""
+    taken, rotate = rotated_by(monkeypatch)
+    cos, sin = tables()
+    q = torch.randn(1, 2, 5, 16)
+    rotate(q, q, cos, sin, *extra)
+    rotate(q, q, cos, sin, unsqueeze_dim=extra[0])
+    rotate(q, q, cos, sin, position_ids=extra[0])
+    assert taken == ["tables"] * 3
+    taken.clear()
+    rotate(q, q, cos, sin), rotate(q, q, cos, sin, 1), rotate(q, q, cos, sin, unsqueeze_dim=1)
+    assert taken == ["positions"] * 3
