@@ -492,7 +492,7 @@ def _family_rope(original: Any, kind: str) -> Any:
             if source is None or not source.stands(cos, sin):
                 if kind == "half" and rope_supported(q, k, cos, sin):
                     return _Rope.apply(q, k, cos, sin)
-            elif rope_at_positions_supported(q, k, source.position_ids, source.inv_freq):
+            elif q.dtype == cos.dtype and rope_at_positions_supported(q, k, source.position_ids, source.inv_freq):
                 return rope_at_positions(q, k, source.position_ids, source.inv_freq, interleaved=kind == "interleaved",
                                          attention_scaling=source.amplitude)
         return original(q, k, cos, sin, *args, **kwargs)

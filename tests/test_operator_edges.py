@@ -431,3 +431,12 @@ def test_other_arguments_go_to_the_family_s_function(extra, monkeypatch):
     taken.clear()
     rotate(q, q, cos, sin), rotate(q, q, cos, sin, 1), rotate(q, q, cos, sin, unsqueeze_dim=1)
     assert taken == ["positions"] * 3
+
+
+def test_tables_of_another_type_go_to_the_family_s_function(monkeypatch):
+    """Under autocast query and key are narrower than the tables; the family's function returns the wider type then."""
+    taken, rotate = rotated_by(monkeypatch)
+    cos, sin = tables()
+    rotate(*[torch.randn(1, 2, 5, 16).bfloat16()] * 2, cos, sin)
+    rotate(*[torch.randn(1, 2, 5, 16)] * 2, cos, sin)
+    assert taken == ["tables", "positions"]
