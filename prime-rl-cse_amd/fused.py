@@ -42,6 +42,14 @@ def _first_derivative(backward: Any) -> Any:
     return run
 
 
+_HERE = {Tensor, nn.Parameter, type(None)}
+
+
+def _spread_out(*tensors: Tensor | None) -> bool:
+    """Whether any is a distributed tensor, whose elements are not where its address says."""
+    return not _HERE.issuperset(map(type, tensors)) and any(hasattr(t, "to_local") for t in tensors)
+
+
 def _through_autograd(*tensors: Tensor | None) -> bool:
     """Whether a call on these goes through its autograd function: a gradient is wanted, or a forward-mode level is open
     (the function refuses dual tensors; a launch by itself would drop their tangents)."""
@@ -327,7 +335,7 @@ def block_norms_supported(x: Tensor, branch: Tensor, post_weight: Tensor | None 
     """Whether `block_norms` takes these tensors: one dtype (bf16 or fp32), one HIP device, rows of at most 8192."""
     given = [t for t in (branch, post_weight, pre_weight, gate) if t is not None]
     if not x.is_cuda or x.ndim < 1 or x.dtype not in (torch.bfloat16, torch.float32) or x.shape != branch.shape \
-            or any(t.dtype != x.dtype or t.device != x.device or hasattr(t, "to_local") for t in given):
+            or any(t.dtype != x.dtype or t.device != x.device for t in given) or _spread_out(x, *given):
         return False
     h = x.shape[-1]
     return 1 <= h <= 8192 and all(w is None or w.shape == (h,) for w in (post_weight, pre_weight))
@@ -695,7 +703,8 @@ class _RopePositions(torch.autograd.Function):
 
 def rope_at_positions_supported(q: Tensor, k: Tensor | None, position_ids: Tensor, inv_freq: Tensor) -> bool:
     """Whether `rope_at_positions` takes these tensors."""
-    if q.ndim != 4 or not q.is_cuda or q.dtype not in (torch.bfloat16, torch.float32):
+    if q.ndim != 4 or not q.is_cuda or q.dtype not in (torch.bfloat16, torch.float32) \
+            or _spread_out(q, k, position_ids, inv_freq):
         return False
     b, _, t, d = q.shape
     if k is not None and (k.ndim != 4 or k.dtype != q.dtype or k.device != q.device

@@ -440,3 +440,24 @@ def test_tables_of_another_type_go_to_the_family_s_function(monkeypatch):
     rotate(*[torch.randn(1, 2, 5, 16).bfloat16()] * 2, cos, sin)
     rotate(*[torch.randn(1, 2, 5, 16)] * 2, cos, sin)
     assert taken == ["tables", "positions"]
+
+
+class SpreadOut(torch.Tensor):
+    """A device tensor whose elements lie somewhere else (as a DTensor's do), as far as the checks can see."""
+
+    is_cuda = property(lambda self: True)
+
+    def to_local(self):
+        raise AssertionError
+
+
+def test_distributed_tensors_are_not_supported():
+    x, w = torch.randn(3, 8), torch.ones(8)
+    far = lambda t: t.as_subclass(SpreadOut)
+    assert not fused.block_norms_supported(far(x), x, w, w)
+    q, pos, freq = torch.randn(1, 2, 5, 8), torch.arange(5), torch.ones(4)
+    assert not fused.rope_at_positions_supported(far(q), None, pos, freq)
+    near = torch.randn(1, 2, 5, 8).as_subclass(type("Near", (torch.Tensor,), {"is_cuda": SpreadOut.is_cuda}))
+    assert fused.rope_at_positions_supported(near, None, pos, freq)
+    for args in ((near, far(q), pos, freq), (near, None, far(pos), freq), (near, None, pos, far(freq))):
+        assert not fused.rope_at_positions_supported(*args)
