@@ -381,7 +381,8 @@ int prl_rope(const void* q, void* q_out, const int64_t* q_strides, int64_t q_hea
  *   the input, then of the output).  q_out / k_out may be q / k themselves under equal strides.
  *   positions  int64 (positions_64 = 1) or int32, element strides over batch and token (a batch stride of 0 is fine)
  *   inv_freq   fp32 or (inv_freq_64 = 1) fp64 [r / 2], contiguous
- * Limits: r even, 2 <= r <= min(D, 8192) (prl_rope_positions_supported), B * T < 2^31 - 64.
+ * Limits: r even, 2 <= r <= min(D, 8192), D <= 2^20 (prl_rope_positions_supported), B * T < 2^31 - 64,
+ * fewer than 2^20 heads of both together.
  */
 int prl_rope_positions_supported(int dtype, int64_t D, int64_t rotary_dim);
 int prl_rope_positions(const void* q, void* q_out, const int64_t* q_strides, int64_t q_heads, const void* k, void* k_out,

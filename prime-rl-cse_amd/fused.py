@@ -706,7 +706,7 @@ def rope_at_positions_supported(q: Tensor, k: Tensor | None, position_ids: Tenso
     if q.ndim != 4 or not q.is_cuda or q.dtype not in (torch.bfloat16, torch.float32) \
             or _spread_out(q, k, position_ids, inv_freq):
         return False
-    b, _, t, d = q.shape
+    b, heads, t, d = q.shape
     if k is not None and (k.ndim != 4 or k.dtype != q.dtype or k.device != q.device
                           or (k.shape[0], k.shape[2], k.shape[3]) != (b, t, d)):
         return False
@@ -715,7 +715,7 @@ def rope_at_positions_supported(q: Tensor, k: Tensor | None, position_ids: Tenso
         return False
     return inv_freq.ndim == 1 and inv_freq.dtype in (torch.float32, torch.float64) and inv_freq.device == q.device \
         and not inv_freq.requires_grad and 1 <= inv_freq.numel() and 2 * inv_freq.numel() <= min(d, 8192) \
-        and b * t < 2**31 - 64
+        and b * t < 2**31 - 64 and d <= 2**20 and heads + (0 if k is None else k.shape[1]) < 2**20
 
 
 def rope_at_positions(q: Tensor, k: Tensor | None, position_ids: Tensor, inv_freq: Tensor, *, interleaved: bool = False,

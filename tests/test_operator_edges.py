@@ -461,3 +461,15 @@ def test_distributed_tensors_are_not_supported():
     assert fused.rope_at_positions_supported(near, None, pos, freq)
     for args in ((near, far(q), pos, freq), (near, None, far(pos), freq), (near, None, pos, far(freq))):
         assert not fused.rope_at_positions_supported(*args)
+
+
+def test_what_the_rotary_entry_refuses_is_not_supported():
+    device = type("Near", (torch.Tensor,), {"is_cuda": SpreadOut.is_cuda})
+    far = lambda *shape: torch.empty(1).expand(shape).as_subclass(device)
+    ok = fused.rope_at_positions_supported
+    pos, freq = torch.arange(3), torch.ones(4)
+    assert ok(far(1, 2, 3, 1 << 20), None, pos, freq) and not ok(far(1, 2, 3, (1 << 20) + 2), None, pos, freq)
+    assert ok(far(1, (1 << 19), 3, 8), far(1, (1 << 19) - 1, 3, 8), pos, freq)
+    assert not ok(far(1, 1 << 19, 3, 8), far(1, 1 << 19, 3, 8), pos, freq)
+    assert not ok(far(1, 1 << 20, 3, 8), None, pos, freq)
+    assert ok(far(0, 2, 3, 8), None, pos, freq)
