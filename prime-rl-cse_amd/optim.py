@@ -240,12 +240,12 @@ def _norm_and_factor(table: np.ndarray, dev: torch.device, kind: int, max_norm: 
 
 @torch.no_grad()
 def grad_norm(grads: Any, norm_type: float = 2.0) -> torch.Tensor:
-    """The norm (2 or inf) of all these tensors together, an fp32 scalar on their device, as
+    """The norm (2 or inf) of all these tensors (or of one) together, an fp32 scalar on their device, as
     torch.nn.utils.get_total_norm; squares are added in fp64 and nothing is copied to the host.  DTensors count with
     all ranks' shards."""
     from . import _capi as C
 
-    grads = list(grads)
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     kind = _norm_kind(norm_type)
     if not grads:
         return torch.tensor(0.0)

@@ -473,3 +473,34 @@ def test_what_the_rotary_entry_refuses_is_not_supported():
     assert not ok(far(1, 1 << 19, 3, 8), far(1, 1 << 19, 3, 8), pos, freq)
     assert not ok(far(1, 1 << 20, 3, 8), None, pos, freq)
     assert ok(far(0, 2, 3, 8), None, pos, freq)
+
+
+def host_clip(monkeypatch):
+    """`clip_grad_norm_` and `grad_norm` up to their launches."""
+    from prime_rl_cse_amd import _capi as C
+    from prime_rl_cse_amd import optim
+
+    on_device(monkeypatch)
+    tables = []
+    monkeypatch.setattr(optim, "_one_device", lambda parts: parts[0].device)
+    monkeypatch.setattr(C, "run", lambda fn, name, dev, *a: tables.append(name))
+    monkeypatch.setattr(C, "stream_ptr", lambda dev: 0)
+    monkeypatch.setattr(C, "check", lambda code, name: None)
+    monkeypatch.setattr(optim, "_norm_and_factor", lambda table, *a: tables.append(table.copy()) or torch.ones(2))
+
+    class Lib:
+        prl_grad_clip = None
+        prl_grad_scale = staticmethod(lambda *a: 0)
+        prl_grad_norm_workspace_bytes = staticmethod(lambda at, n: 8)
+
+    monkeypatch.setattr(C, "load", lambda: Lib)
+    return optim, tables
+
+
+@pytest.mark.parametrize("shape", [(), (7,), (4, 5), (2, 3, 4)])
+def test_the_norm_of_one_tensor(shape, monkeypatch):
+    optim, tables = host_clip(monkeypatch)
+    t = torch.randn(shape)
+    optim.grad_norm(t)
+    optim.grad_norm(t.t() if t.ndim == 2 else t)
+    assert [(int(p["x"]), int(p["n"])) for table in tables for p in table] == [(t.data_ptr(), t.numel())] * 2
