@@ -203,6 +203,15 @@ def _pieces(grads: list[torch.Tensor], in_place: bool) -> np.ndarray:
     return table
 
 
+def _written(tensors: list[torch.Tensor]) -> None:
+    """Counts a write to each of them, as torch's in-place operations do: a graph that has kept one notices."""
+    count = torch.autograd.graph.increment_version
+    try:
+        count(tensors)
+    except RuntimeError:  # (inference tensors count none; one counted twice is no harm)
+        count([t for t in tensors if not t.is_inference()])
+
+
 def _norm_kind(norm_type: float) -> int:
     from . import _capi as C
 
@@ -288,12 +297,16 @@ def clip_grad_norm_(parameters: Any, max_norm: float, norm_type: float = 2.0,
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
         C.run(lib.prl_grad_clip, "prl_grad_clip", dev, at, n, kind, float(max_norm), norm.data_ptr(), ws.data_ptr(), size,
               C.stream_ptr(dev))
+        _written(grads)
         return norm
     with C.on_device(dev), C.timed("prl_grad_clip", dev):
         out = _norm_and_factor(table, dev, kind, float(max_norm), groups)
         if error_if_nonfinite and not math.isfinite(float(out[0])):
             raise RuntimeError(f"The total norm of order {norm_type} of the gradients is not finite, so they cannot be clipped")
         C.check(lib.prl_grad_scale(at, n, out.data_ptr() + 4, C.stream_ptr(dev)), "prl_grad_scale")
+    _written(grads)
+    if parts is not grads:
+        _written(parts)
     return out[0]
 
 

@@ -504,3 +504,23 @@ def test_the_norm_of_one_tensor(shape, monkeypatch):
     optim.grad_norm(t)
     optim.grad_norm(t.t() if t.ndim == 2 else t)
     assert [(int(p["x"]), int(p["n"])) for table in tables for p in table] == [(t.data_ptr(), t.numel())] * 2
+
+
+@pytest.mark.parametrize("check", [False, True])
+def test_clipping_counts_as_a_write(check, monkeypatch):
+    """A graph that has kept a gradient refuses its backward after the gradient was scaled, as after torch's own clipping."""
+    optim, _ = host_clip(monkeypatch)
+    params = [torch.nn.Parameter(torch.zeros(4)) for _ in range(3)]
+    for p in params[:2]:
+        p.grad = torch.randn(4)
+    w = torch.ones(4, requires_grad=True)
+    kept = (params[1].grad * w).sum()
+    optim.clip_grad_norm_(params, 1.0, error_if_nonfinite=check)
+    assert [p.grad._version for p in params[:2]] == [1, 1]
+    with pytest.raises(RuntimeError):
+        kept.backward()
+    with torch.inference_mode():  # (tensors that count no writes)
+        quiet = torch.nn.Parameter(torch.zeros(4))
+        quiet.grad = torch.randn(4)
+        optim.clip_grad_norm_([quiet, params[0]], 1.0, error_if_nonfinite=check)
+    assert params[0].grad._version == 2
