@@ -538,9 +538,12 @@ def _probe_rotary(rotate: Any, module: nn.Module, size: int) -> str | None:
     whole) that way, by position times the module's `inv_freq`; None otherwise."""
     import copy
 
-    rotary = copy.deepcopy(module)
-    rotary.forward = types.MethodType(type(rotary).forward, rotary)
-    rotary = rotary.cpu().float()
+    try:
+        rotary = copy.deepcopy(module)
+        rotary.forward = types.MethodType(type(rotary).forward, rotary)
+        rotary = rotary.cpu().float()
+    except Exception:  # (it holds something that has no copy)
+        return None
     gen = torch.Generator().manual_seed(0)
     randn = lambda *shape: torch.randn(shape, generator=gen, dtype=torch.float32, device="cpu")
     pos = torch.tensor([[3, 4, 5, 11, 2]], device="cpu")

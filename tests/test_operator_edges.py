@@ -524,3 +524,21 @@ def test_clipping_counts_as_a_write(check, monkeypatch):
         quiet.grad = torch.randn(4)
         optim.clip_grad_norm_([quiet, params[0]], 1.0, error_if_nonfinite=check)
     assert params[0].grad._version == 2
+
+
+@pytest.mark.parametrize("both", [False, True])
+def test_a_rotary_module_that_cannot_be_copied_is_left_alone(both):
+    import sys
+
+    model = sandwich("Glm4")
+    rotary = model.model.rotary_emb
+    if not both:
+        model.extra = copy.deepcopy(rotary)
+    rotary.open_file = (i for i in range(2))
+    home = sys.modules[type(model).__module__]
+    found = fused._rope_kind(home, model)
+    assert found is None if both else found == ("interleaved", [model.extra])
+    try:
+        fused.fuse_model(model)
+    finally:
+        fused.unfuse_model(model)
