@@ -240,11 +240,12 @@ def _pitched(x: Tensor, h: int) -> Tensor:
     return x
 
 
-def _fresh_rows(x: Tensor) -> Tensor:
+def _fresh_rows(x: Tensor, how_many: int = 2) -> list[Tensor]:
     """Memory for rows like x's, h apart.  (`empty_like` is the cheapest call, but of rows that overlap it makes rows one
     element apart.)"""
-    out = torch.empty_like(x)
-    return out if out.stride(0) == x.shape[1] else torch.empty_like(x, memory_format=torch.contiguous_format)
+    if x.stride(0) >= x.shape[1]:
+        return [torch.empty_like(x) for _ in range(how_many)]
+    return [torch.empty_like(x, memory_format=torch.contiguous_format) for _ in range(how_many)]
 
 
 def _gate_rows(gate: Tensor, lead: tuple[int, ...], h: int) -> tuple[int, Tensor]:
@@ -285,8 +286,7 @@ class _BlockNorms(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, branch: Tensor, w_post: Tensor | None, w_pre: Tensor | None, gate: Tensor | None,
                 kind: int, scale: float, offset: float, eps_post: float, eps_pre: float):
-        hidden = _fresh_rows(x)
-        normed = None if w_pre is None else _fresh_rows(x)
+        hidden, normed = (*_fresh_rows(x, 1), None) if w_pre is None else _fresh_rows(x)
         rstd = torch.empty(2 * x.shape[0], dtype=torch.float32, device=x.device)  # of the branch, then of the sum
         _launch_block_norms(x, branch, w_post, w_pre, gate, kind, scale, offset, eps_post, eps_pre, hidden, normed, rstd)
         ctx.save_for_backward(x, branch, w_post, w_pre, gate, rstd)
@@ -309,7 +309,7 @@ class _BlockNorms(torch.autograd.Function):
         gh = None if gh is None else _pitched(gh, h)
         gy = None if gy is None else _pitched(gy, h)
         need = ctx.needs_input_grad
-        gx, gb = _fresh_rows(x), _fresh_rows(x)
+        gx, gb = _fresh_rows(x)
         g1 = torch.empty_like(w_post) if w_post is not None and need[2] else None
         g2 = torch.empty_like(w_pre) if w_pre is not None and need[3] else None
         gg = torch.empty(gate.shape, dtype=x.dtype, device=dev) if gate is not None and need[4] else None
@@ -333,12 +333,17 @@ class _BlockNorms(torch.autograd.Function):
 def block_norms_supported(x: Tensor, branch: Tensor, post_weight: Tensor | None = None, pre_weight: Tensor | None = None,
                           gate: Tensor | None = None) -> bool:
     """Whether `block_norms` takes these tensors: one dtype (bf16 or fp32), one HIP device, rows of at most 8192."""
-    given = [t for t in (branch, post_weight, pre_weight, gate) if t is not None]
-    if not x.is_cuda or x.ndim < 1 or x.dtype not in (torch.bfloat16, torch.float32) or x.shape != branch.shape \
-            or any(t.dtype != x.dtype or t.device != x.device for t in given) or _spread_out(x, *given):
+    dtype, device, shape = x.dtype, x.device, x.shape
+    if not x.is_cuda or not shape or dtype not in (torch.bfloat16, torch.float32) or shape != branch.shape:
         return False
-    h = x.shape[-1]
-    return 1 <= h <= 8192 and all(w is None or w.shape == (h,) for w in (post_weight, pre_weight))
+    for t in (branch, post_weight, pre_weight, gate):
+        if t is not None and (t.dtype != dtype or t.device != device):
+            return False
+    if _spread_out(x, branch, post_weight, pre_weight, gate):
+        return False
+    h = shape[-1]
+    return 1 <= h <= 8192 and (post_weight is None or post_weight.shape == (h,)) \
+        and (pre_weight is None or pre_weight.shape == (h,))
 
 
 def block_norms(x: Tensor, branch: Tensor, post_weight: Tensor | None = None, pre_weight: Tensor | None = None, *,
@@ -373,7 +378,7 @@ def block_norms(x: Tensor, branch: Tensor, post_weight: Tensor | None = None, pr
     if _through_autograd(x, branch, w1, w2, gate):
         hidden, normed = _BlockNorms.apply(*args)
     else:
-        hidden, normed = _fresh_rows(x), None if w2 is None else _fresh_rows(x)
+        hidden, normed = (*_fresh_rows(x, 1), None) if w2 is None else _fresh_rows(x)
         _launch_block_norms(*args, hidden, normed, None)
     if len(shape) != 2:
         hidden, normed = hidden.view(shape), None if normed is None else normed.view(shape)
@@ -706,19 +711,25 @@ class _RopePositions(torch.autograd.Function):
 
 def rope_at_positions_supported(q: Tensor, k: Tensor | None, position_ids: Tensor, inv_freq: Tensor) -> bool:
     """Whether `rope_at_positions` takes these tensors."""
-    if q.ndim != 4 or not q.is_cuda or q.dtype not in (torch.bfloat16, torch.float32) \
+    dtype, device = q.dtype, q.device
+    if q.ndim != 4 or not q.is_cuda or dtype not in (torch.bfloat16, torch.float32) \
             or _spread_out(q, k, position_ids, inv_freq):
         return False
     b, heads, t, d = q.shape
-    if k is not None and (k.ndim != 4 or k.dtype != q.dtype or k.device != q.device
-                          or (k.shape[0], k.shape[2], k.shape[3]) != (b, t, d)):
+    if k is not None:
+        if k.ndim != 4 or k.dtype != dtype or k.device != device:
+            return False
+        kb, more, kt, kd = k.shape
+        if (kb, kt, kd) != (b, t, d):
+            return False
+        heads += more
+    if position_ids.dtype not in (torch.int64, torch.int32) or position_ids.device != device \
+            or position_ids.shape not in ((b, t), (1, t), (t,)):
         return False
-    if position_ids.dtype not in (torch.int64, torch.int32) or position_ids.device != q.device \
-            or tuple(position_ids.shape) not in ((b, t), (1, t), (t,)):
-        return False
-    return inv_freq.ndim == 1 and inv_freq.dtype in (torch.float32, torch.float64) and inv_freq.device == q.device \
-        and not inv_freq.requires_grad and 1 <= inv_freq.numel() and 2 * inv_freq.numel() <= min(d, 8192) \
-        and b * t < 2**31 - 64 and d <= 2**20 and heads + (0 if k is None else k.shape[1]) < 2**20
+    pairs = inv_freq.numel()
+    return inv_freq.ndim == 1 and inv_freq.dtype in (torch.float32, torch.float64) and inv_freq.device == device \
+        and not inv_freq.requires_grad and 1 <= pairs and 2 * pairs <= min(d, 8192) \
+        and b * t < 2**31 - 64 and d <= 2**20 and heads < 2**20
 
 
 def rope_at_positions(q: Tensor, k: Tensor | None, position_ids: Tensor, inv_freq: Tensor, *, interleaved: bool = False,

@@ -144,8 +144,7 @@ def _is_one_run(g: torch.Tensor) -> bool:
 
 
 def _overlap(at: np.ndarray, size: np.ndarray) -> bool:
-    """Whether any two runs of `size` bytes at these addresses share memory (empty runs share none)."""
-    at, size = at[size > 0], size[size > 0]
+    """Whether any two runs of `size` bytes (none empty) at these addresses share memory."""
     order = np.argsort(at)
     return bool(((at + size)[order[:-1]] > at[order[1:]]).any())
 
@@ -162,8 +161,8 @@ def clip_grad_norm_supported(grads: list[torch.Tensor]) -> bool:
     if len(index) != 1 or index == {-1} or not set(map(_DTYPE, parts)) <= _TYPES \
             or not all(g.layout is torch.strided and _is_one_run(g) for g in parts):
         return False
-    at = np.array(list(map(torch.Tensor.data_ptr, parts)), dtype=np.int64)
-    return not _overlap(at, np.array([g.numel() * g.element_size() for g in parts], dtype=np.int64))
+    runs = np.array([(g.data_ptr(), g.nbytes) for g in parts if g.numel()], dtype=np.int64).reshape(-1, 2)
+    return not _overlap(runs[:, 0], runs[:, 1])
 
 
 _GRAD, _DTYPE = operator.attrgetter("grad"), operator.attrgetter("dtype")
@@ -284,10 +283,11 @@ def clip_grad_norm_(parameters: Any, max_norm: float, norm_type: float = 2.0,
     kind = _norm_kind(norm_type)
     if not grads:
         return torch.tensor(0.0)
-    groups = _sharding(grads)
+    plain = _all_plain(grads)
+    groups = [] if plain else _sharding(grads)
     if groups is None:
         raise ValueError("clip_grad_norm_: plain gradients, or DTensors of one mesh placed alike (sharded or replicated)")
-    parts = _local_parts(grads)
+    parts = grads if plain else _local_parts(grads)
     dev = _one_device(parts)
     table = _pieces(parts, in_place=True)
     lib, at, n = C.load(), table.ctypes.data, len(table)
