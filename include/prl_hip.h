@@ -554,7 +554,7 @@ int prl_adamw_flat(float* param, float* grad, float* exp_avg, float* exp_avg_sq,
  * prl_grad_norm_finish joins n_parts partial totals (e.g. the one all ranks have reduced) and gives total, norm and
  * coef.  prl_grad_scale multiplies every piece by coef[0] in place; where that is exactly 1 nothing is touched.
  * prl_grad_clip is prl_grad_norm and prl_grad_scale in one call (and one launch fewer), for gradients of one process.
- * Squares are added in fp64 in an order fixed by the sizes.  A NaN anywhere gives NaN, an infinity an infinite norm.
+ * Squares are added in fp64 in an order fixed by the pieces' sizes and addresses.  A NaN anywhere gives NaN, an infinity an infinite norm.
  */
 #define PRL_NORM_L2 0
 #define PRL_NORM_MAX 1

@@ -1,14 +1,16 @@
 // The global norm of many gradient tensors, and their clipping, as torch.nn.utils.clip_grad_norm_ does it for the
 // reference (src/prime_rl/trainer/rl/train.py:336-338):
 //     N = sqrt(sum g^2)  or  max |g|,    c = min(1, max_norm / (N + 1e-6)),    g <- g c
-// Two passes over the gradients; where c is exactly 1 the second returns at once.  Bound by HBM: 1.8 GB of fp32 take
-// 290 us to read (6.2 TB/s) and 623 us to scale (5.8).  Both go past the caches (non-temporal: 1029 -> 875 us for the two
-// together); keeping the end of the first pass in the last-level cache for the second gained nothing.
+// Two passes over the gradients; where c is exactly 1 the second touches none.  Bound by HBM: 1.8 GB of fp32 in 310
+// tensors take 874 us when they are clipped (6.1 TB/s over two reads and a write), 325 when there is nothing to clip
+// (5.5).  Both passes go past the caches (non-temporal: 1029 -> 875 us); keeping the end of the first in the last-level
+// cache for the second gained nothing.
 //
 // The tensors' addresses and lengths travel in the launch itself, up to kClipPieces of them each: nothing is copied to
 // the device, the calls are legal under stream capture, and no table outlives them.  Pieces are cut into chunks; a
 // workgroup takes every so-manieth of them.  Squares are formed and added in fp64: no overflow for any fp32
-// gradient, and the order of the sums is fixed by the sizes alone.
+// gradient.  The order of the sums is fixed by the tensors' sizes and places in memory (which of them touch, where each
+// starts within 16 bytes): the same buffers give the same bits, others may differ in the last of 64.
 #include "prl_common.h"
 
 namespace prl {
@@ -191,7 +193,9 @@ __global__ __launch_bounds__(kClipThreads) void k_grad_scale(const ClipTable t, 
   clip_scale(t, *coef);
 }
 // The scaling with the finish in it: every workgroup joins the partial values itself, in the same order, which is
-// cheaper than a launch between the two (2 us against 4.5 with nothing to clip).
+// cheaper than a launch between the two (2 us against 4.5 with nothing to clip) for few launches' partial values.  With
+// many tensors the joining shows: 706 of bf16, 1.9 GB, five launches of partial values, take 624 us with nothing to clip,
+// about twice the time of their read.  There is no other form for that yet.
 template <bool MAX>
 __global__ __launch_bounds__(kClipThreads) void k_grad_clip(const ClipTable t, const double* __restrict__ part, int nparts,
                                                             float max_norm, float* __restrict__ norm) {
