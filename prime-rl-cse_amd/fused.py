@@ -1003,7 +1003,8 @@ class _Carry:
     normalisation kernel.  Bound to the identity of the returned tensor: a reader that is handed anything else
     while a branch is pending fails instead of computing without it."""
 
-    def __init__(self) -> None:
+    def __init__(self, readers: list[nn.Module]) -> None:
+        self.readers = readers  # the layers in their order, then the final norm
         self.clear()
 
     def clear(self) -> None:
@@ -1053,7 +1054,7 @@ def _add_norm(norm: nn.Module, x: Tensor, branch: Tensor, inside: bool = False) 
 def _hands_on(layer: nn.Module) -> bool:
     """Whether a layer may leave its last addition to the next reader: nobody looks at what it returns, nor at what
     that reader is given."""
-    return not _watched(layer, arrivals=False) and not _watched(layer._prl_reader[0], arrivals=False)
+    return not any(_watched(m, arrivals=False) for m in layer._prl_carry.readers[layer._prl_at : layer._prl_at + 2])
 
 
 def _fused_layer_forward(self: nn.Module, hidden_states: Tensor, attention_mask: Tensor | None = None,
@@ -1330,10 +1331,9 @@ def enable_residual_carry(model: nn.Module, on: bool = True) -> int:
             if m is not None and hasattr(m, "_prl_carry"):
                 m._prl_carry = None
         return 0
-    carry = _Carry()
+    carry = _Carry([*layers, final])
     for i, m in enumerate(layers):
-        m._prl_carry, m._prl_first = carry, i == 0
-        m._prl_reader = (layers[i + 1] if i + 1 < len(layers) else final,)  # (in a tuple: not a child module)
+        m._prl_carry, m._prl_first, m._prl_at = carry, i == 0, i
     final._prl_carry = carry
     return len(layers)
 
@@ -1651,7 +1651,7 @@ def unfuse_model(model: nn.Module) -> None:
         if hasattr(module, "_prl_torch_forward"):
             module.forward = module._prl_torch_forward
             del module._prl_torch_forward
-            for attr in ("_prl_qkv", "_prl_carry", "_prl_first", "_prl_reader", "_prl_steps"):
+            for attr in ("_prl_qkv", "_prl_carry", "_prl_first", "_prl_at", "_prl_steps"):
                 if hasattr(module, attr):
                     delattr(module, attr)
 

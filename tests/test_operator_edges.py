@@ -189,7 +189,7 @@ def test_hooks_on_layers_see_whole_hidden_states(name, monkeypatch):
         handle.remove()
     finally:
         fused.unfuse_model(model)
-    assert not hasattr(model.model.layers[0], "_prl_reader")
+    assert not hasattr(model.model.layers[0], "_prl_at")
 
 
 def test_backward_hooks_on_norms_run(monkeypatch):
@@ -542,3 +542,22 @@ def test_a_rotary_module_that_cannot_be_copied_is_left_alone(both):
         fused.fuse_model(model)
     finally:
         fused.unfuse_model(model)
+
+
+def test_a_deep_model_that_carries_can_be_copied():
+    class Inner(torch.nn.Module):
+        def __init__(self, layers, norm):
+            super().__init__()
+            self.layers, self.norm = torch.nn.ModuleList(layers), norm
+
+    model = torch.nn.Module()
+    base = sandwich("Qwen3").model
+    model.model = Inner([copy.deepcopy(base.layers[0]) for _ in range(300)], base.norm)
+    fused.fuse_model(model)
+    assert fused.enable_residual_carry(model) == 300
+    other = copy.deepcopy(model)
+    first, last = other.model.layers[0], other.model.layers[-1]
+    assert first._prl_carry is last._prl_carry is other.model.norm._prl_carry is not model.model.norm._prl_carry
+    assert fused._hands_on(first) and fused._hands_on(last)
+    other.model.norm.register_forward_hook(lambda *a: None)
+    assert fused._hands_on(first) and not fused._hands_on(last) and fused._hands_on(model.model.layers[-1])
