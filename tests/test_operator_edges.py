@@ -561,3 +561,33 @@ def test_a_deep_model_that_carries_can_be_copied():
     assert fused._hands_on(first) and fused._hands_on(last)
     other.model.norm.register_forward_hook(lambda *a: None)
     assert fused._hands_on(first) and not fused._hands_on(last) and fused._hands_on(model.model.layers[-1])
+
+
+def test_hooks_that_wait_for_weights_leave_the_carry(monkeypatch):
+    """The exchange's own pre-hooks (`Replica`): on layers, the final norm, and norms by themselves."""
+    from types import SimpleNamespace
+
+    from prime_rl_cse_amd.replica import Replica
+
+    model = sandwich("Glm4")
+    calls = stepwise(monkeypatch)
+    fused.fuse_model(model)
+    try:
+        fused.enable_residual_carry(model)
+        want = logits(model)
+        expected = list(calls)
+        params = list(model.parameters())
+        inside = {id(p) for p in model.model.layers[1].parameters()}
+        names = {id(p): n for n, p in model.named_parameters()}
+        # the second layer cut: its norms in a bucket of their own, so that they get hooks of their own
+        bucket_of = [2 if id(p) in inside and "layernorm" in names[id(p)] else 1 if id(p) in inside else 0 for p in params]
+        waited = []
+        state = SimpleNamespace(params=params, bucket_of=bucket_of, buckets=[0, 1, 2], wait_gathered=waited.append)
+        Replica._hook_weight_arrival(SimpleNamespace(model=model, state=state))
+        assert all(fused._hands_on(m) for m in model.model.layers)
+        calls.clear()
+        assert close(logits(model), want)
+        # each of the cut layer's four norms was waited for (called as a module where it has its own hook)
+        assert waited.count(2) == 4 and len(calls) < len(expected)
+    finally:
+        fused.unfuse_model(model)
