@@ -6,7 +6,7 @@ import torch
 
 import prime_rl_cse_amd as prl  # noqa: F401
 from prime_rl_cse_amd import fused
-from tests.test_gpu_block_norms import E1, E2, HALF_STEP, U, bounds
+from tests.test_gpu_block_norms import E1, E2, HALF_STEP, U, bounds, make
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -67,3 +67,35 @@ def test_no_rows_with_every_gate(gate):
     out = fused.block_norms(x, x, w, w, gate=g)
     for grad, leaf in zip(torch.autograd.grad(out, leaves, [torch.empty(0, 48, device=DEV)] * 2), leaves):
         assert grad.shape == leaf.shape and not bool(grad.any())
+
+
+def placed(v, pitch, at):
+    """v's values in rows `pitch` apart, `at` elements behind an allocation's start."""
+    rows, h = v.shape
+    out = torch.full((rows * pitch + at,), float("nan"), device=DEV, dtype=v.dtype)[at:].view(rows, pitch)[:, :h]
+    return out.copy_(v)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("gate", [None, "channel", "token", "full"])
+@pytest.mark.parametrize("rows, h, pitch, at", [(9, 264, 272, 8), (9, 264, 265, 0), (40, 1000, 1001, 3), (5, 1531, 1600, 1),
+                                                (300, 2048, 6144, 2048), (3, 8191, 8200, 5), (4, 5000, 5004, 4)])
+def test_norms_of_rows_inside_wider_ones(rows, h, pitch, at, gate, dtype):
+    """Rows where they lie, of another pitch for each input, at places of any alignment; what lies between is not read."""
+    t = make(rows, h, dtype, gate, True, True, seed=4)
+    for i, k in enumerate(("x", "b", "gh", "gy", "g")):
+        if t[k] is not None and t[k].shape == (rows, h):
+            t[k] = placed(t[k], pitch + 8 * i, at)
+        elif t[k] is not None:  # a gate per row or channel, every third place
+            t[k] = torch.full((3 * t[k].numel(),), float("nan"), device=DEV, dtype=dtype)[::3].copy_(t[k].view(-1)).view(
+                t[k].shape)
+    leaves = {k: t[k].detach().requires_grad_(True) for k in ("x", "b", "w1", "w2", "g") if t[k] is not None}
+    assert leaves["x"].stride(0) == pitch
+    out = fused.block_norms(leaves["x"], leaves["b"], leaves["w1"], leaves["w2"], gate=leaves.get("g"), scale=0.5, eps=E1,
+                            pre_eps=E2)
+    got = dict(zip(("h", "y", *leaves), (*out, *torch.autograd.grad(out, list(leaves.values()), [t["gh"], t["gy"]]))))
+    want, mag = bounds(t, 0.5, 0.0, rows)
+    for name, v in got.items():
+        steps = (64 if name in "hy" else 160) + (72 + rows // 256 + 1 if name in ("w1", "w2", "g") else 0)
+        tol = HALF_STEP[dtype] * want[name].abs() * (1 + 2.0**-10) + steps * U * mag[name] + 1e-30
+        assert v.shape == want[name].shape and bool(((v.double() - want[name]).abs() <= tol).all()), name
