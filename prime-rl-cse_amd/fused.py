@@ -1320,7 +1320,8 @@ def enable_residual_carry(model: nn.Module, on: bool = True) -> int:
     to the final norm) instead of adding it itself.  Only for a model whose layers run back to back in one
     process-local forward: not under per-layer activation checkpointing (a re-run layer would not get the branch
     again) nor under per-layer FSDP (its pre-backward hook hangs on the layer's returned tensor, and the MLP's
-    backward can run before it).  A layer that hooks hang on, or on whose reader they do, adds by itself.  Returns the number of layers that carry (0: the model is not shaped for it)."""
+    backward can run before it).  A layer that hooks hang on, or on whose reader they do, adds by itself.  Returns the
+    number of layers that carry (0: the model is not shaped for it)."""
     inner = getattr(model, "model", None)
     layers = list(getattr(inner, "layers", []) or [])
     final = getattr(inner, "norm", None)
@@ -1634,7 +1635,8 @@ def fuse_model(model: nn.Module) -> dict[str, int]:
             done["qkv"] += 1
             if hasattr(module, "q_norm") and hasattr(module, "k_norm") and hasattr(module, "head_dim") \
                     and hasattr(module, "o_proj") and not hasattr(module, "_prl_torch_forward") \
-                    and (whole_heads_in_halves or not hasattr(home, "apply_rotary_pos_emb")):
+                    and (whole_heads_in_halves or not hasattr(home, "apply_rotary_pos_emb")) \
+                    and 1.0 not in (_norm_form(module.q_norm), _norm_form(module.k_norm)):
                 module._prl_torch_forward = module.forward
                 module.forward = types.MethodType(_fused_attention_forward, module)
     return done

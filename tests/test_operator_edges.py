@@ -591,3 +591,35 @@ def test_hooks_that_wait_for_weights_leave_the_carry(monkeypatch):
         assert waited.count(2) == 4 and len(calls) < len(expected)
     finally:
         fused.unfuse_model(model)
+
+
+def attention_blocks_taken(model, monkeypatch):
+    """How many attention blocks of one forward the fused form asks for their stacked projection."""
+    asked = []
+    monkeypatch.setattr(fused, "_stackable", lambda x, *linears: asked.append(len(linears)))
+    model(input_ids=torch.arange(12)[None], position_ids=torch.arange(12)[None])
+    return asked.count(3)
+
+
+def wide_heads():
+    from tests.test_fuse_families import tiny
+
+    return tiny("Qwen3", head_dim=128, num_attention_heads=2, num_key_value_heads=1)
+
+
+def test_a_query_norm_that_adds_one_keeps_the_attention_block_s_own_forward(monkeypatch):
+    model = wide_heads()
+    fused.fuse_model(model)
+    assert hasattr(model.model.layers[0].self_attn, "_prl_torch_forward")
+    fused.unfuse_model(model)
+
+    class FromOneRMSNorm(type(model.model.norm)):
+        def forward(self, x):
+            return x * torch.rsqrt((x * x).mean(-1, keepdim=True) + self.variance_epsilon) * (1.0 + self.weight)
+
+    model.model.layers[0].self_attn.k_norm.__class__ = FromOneRMSNorm
+    fused.fuse_model(model)
+    try:
+        assert [hasattr(m.self_attn, "_prl_torch_forward") for m in model.model.layers] == [False, True]
+    finally:
+        fused.unfuse_model(model)
