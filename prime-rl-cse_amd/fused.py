@@ -1483,7 +1483,8 @@ def _fused_attention_forward(self: nn.Module, hidden_states: Tensor, position_em
         and qn.variance_epsilon == kn.variance_epsilon and not hasattr(qn.weight, "to_local") \
         and cos.dtype == x.dtype and cos.shape == (1, x.shape[1], 128) and cos.stride(-1) == 1 \
         and sin.stride() == cos.stride() and not cos.requires_grad \
-        and (cos.stride(1) * cos.element_size()) % 16 == 0 and cos.data_ptr() % 16 == 0 and sin.data_ptr() % 16 == 0
+        and (cos.stride(1) * cos.element_size()) % 16 == 0 and cos.data_ptr() % 16 == 0 and sin.data_ptr() % 16 == 0 \
+        and not _watched(qn) and not _watched(kn)
     from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 
     stacked = _stackable(x, self.q_proj, self.k_proj, self.v_proj) if ok else None

@@ -623,3 +623,16 @@ def test_a_query_norm_that_adds_one_keeps_the_attention_block_s_own_forward(monk
         assert [hasattr(m.self_attn, "_prl_torch_forward") for m in model.model.layers] == [False, True]
     finally:
         fused.unfuse_model(model)
+
+
+@pytest.mark.parametrize("which", ["q_norm", "k_norm"])
+def test_an_attention_block_with_hooks_on_its_norms_runs_its_own_forward(which, monkeypatch):
+    model = wide_heads()
+    fused.fuse_model(model)
+    try:
+        assert attention_blocks_taken(model, monkeypatch) == 2
+        seen = []
+        getattr(model.model.layers[1].self_attn, which).register_forward_hook(lambda *a: seen.append(1))
+        assert attention_blocks_taken(model, monkeypatch) == 1 and len(seen) == 1
+    finally:
+        fused.unfuse_model(model)
